@@ -273,6 +273,58 @@ int optimi_b200_ranger(int n_tensors, void* const* params, void* const* grads, v
                        int do_lookahead, double alpha, int decouple_wd, int kahan_sum, int update_parameters,
                        void* stream);
 
+/* Activations kept in 8 bits for the backward pass.  No counterpart in the reference: its gradient release
+ * (optimi/gradientrelease.py:13-61) leaves activations as what a training step holds in memory.
+ *
+ * Format.  An activation of `rows` tokens and `cols` channels is held as int8 codes, row by row with a
+ * pitch of `code_pitch` bytes (a multiple of 32, at least cols rounded up to 32; base 16-byte aligned;
+ * the columns from cols up to that multiple hold zeros), and one exponent byte e for every 32
+ * neighbouring channels of a token (`exponent_pitch` bytes from row to row).  A value is
+ * code * 2^(e - 127), codes from -127 to 127; e = 0 is a group of zeros, e = 255 a group that held an
+ * infinity or a NaN and reads back as NaNs.  2^(e - 127) is the smallest power of two of which the
+ * group's largest magnitude, rounded to nearest even, is at most 127, kept within 2^-126 .. 2^121
+ * (float16: 2^-24 .. 2^9), so that every restored value is exact in its type.
+ *
+ * Shared rules: x_stride, grad_stride, ... are element counts from row to row, rows themselves are
+ * contiguous; results are contiguous; all buffers live on the current device; dimensions reach 2^31-1
+ * and offsets 64 bits.  The calls carry no step-dependent scalars and may be captured into a CUDA graph.
+ *
+ * optimi_b200_compress, optimi_b200_decompress: to the format and back.  `channel_scale` (NULL, or `cols`
+ * values of type `dtype`) multiplies the restored columns in fp32 before the one rounding. */
+int optimi_b200_compress(const void* x, int64_t x_stride, int64_t rows, int64_t cols, int dtype, void* codes,
+                         int64_t code_pitch, void* exponents, int64_t exponent_pitch, void* stream);
+int optimi_b200_decompress(const void* codes, int64_t code_pitch, const void* exponents, int64_t exponent_pitch,
+                           const void* channel_scale, int64_t rows, int64_t cols, int dtype, void* out, void* stream);
+
+/* Residual addition and RMS norm with an output in 8 bits.  h = round(x + residual) (`sum`; both NULL: h = x),
+ * xn = h / sqrt(mean(h^2) + eps), y = round(xn * weight) (NULL: 1).  With codes, exponents and rstd (all
+ * or none) the 8-bit form of xn (without the weight) and 1 / sqrt(mean(h^2) + eps) are written too: what
+ * optimi_b200_rms_norm_backward reads.
+ *
+ * Backward: g = grad * weight, grad_input = rstd * (g - xn * mean(g * xn)) + grad_sum, grad_weight = sum
+ * over the rows of grad * xn.  grad_input is the gradient of x and of the residual alike; grad_sum (NULL:
+ * none) is the gradient that arrives at h.  grad_input or grad_weight may be NULL.  `workspace`
+ * (with grad_weight): DEVICE scratch of optimi_b200_rms_norm_backward_workspace_bytes(rows, cols) bytes,
+ * 16-byte aligned.  Sums are taken in a fixed order. */
+int optimi_b200_rms_norm(const void* x, int64_t x_stride, const void* residual, int64_t residual_stride, const void* weight,
+                         int64_t rows, int64_t cols, double eps, int dtype, void* y, void* sum, void* codes, int64_t code_pitch,
+                         void* exponents, int64_t exponent_pitch, float* rstd, void* stream);
+size_t optimi_b200_rms_norm_backward_workspace_bytes(int64_t rows, int64_t cols);
+int optimi_b200_rms_norm_backward(const void* grad, int64_t grad_stride, const void* grad_sum, int64_t grad_sum_stride,
+                                  const void* codes, int64_t code_pitch, const void* exponents, int64_t exponent_pitch,
+                                  const float* rstd, const void* weight, int64_t rows, int64_t cols, int dtype, void* grad_input,
+                                  void* grad_weight, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Weight gradient of a linear layer whose input is held in 8 bits: grad_weight[o][c] = channel_scale[c] *
+ * sum over t of grad[t][o] * X[t][c], rounded once (`channel_scale` NULL: 1).  dtype (of grad,
+ * channel_scale and grad_weight): OPTIMI_BF16 or OPTIMI_F16.  `workspace`: DEVICE scratch of
+ * optimi_b200_weight_gradient_workspace_bytes(rows, outputs, channels) bytes, 16-byte aligned. */
+size_t optimi_b200_weight_gradient_workspace_bytes(int64_t rows, int64_t outputs, int64_t channels);
+int optimi_b200_weight_gradient(const void* grad, int64_t grad_stride, const void* codes, int64_t code_pitch,
+                                const void* exponents, int64_t exponent_pitch, const void* channel_scale, int64_t rows,
+                                int64_t outputs, int64_t channels, int dtype, void* grad_weight, void* workspace,
+                                size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

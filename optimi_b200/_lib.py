@@ -31,7 +31,17 @@ SIGNATURES = {
     "optimi_b200_radam": [_I] + [_P] * 5 + [_P, _I] + [_D] * 6 + [_I, _D] + [_I] * 3 + [_P],
     "optimi_b200_ranger": [_I] + [_P] * 6 + [_P, _I] + [_D] * 6 + [_I, _D, _I, _D] + [_I] * 3 + [_P],
 }
-EXPORTS = list(SIGNATURES) + ["optimi_b200_push_begin", "optimi_b200_push_end", "optimi_b200_pull_begin", "optimi_b200_pull_end", "optimi_b200_last_error", "optimi_b200_version", "optimi_b200_launch_count", "optimi_b200_stableadamw_workspace_bytes",
+_L, _Z = ctypes.c_int64, ctypes.c_size_t
+# the activation entry points (plain device pointers instead of lists)
+ACTIVATION_SIGNATURES = {
+    "optimi_b200_compress": [_P, _L, _L, _L, _I, _P, _L, _P, _L, _P],
+    "optimi_b200_decompress": [_P, _L, _P, _L, _P, _L, _L, _I, _P, _P],
+    "optimi_b200_rms_norm": [_P, _L, _P, _L, _P, _L, _L, _D, _I, _P, _P, _P, _L, _P, _L, _P, _P],
+    "optimi_b200_rms_norm_backward": [_P, _L, _P, _L, _P, _L, _P, _L, _P, _P, _L, _L, _I, _P, _P, _P, _Z, _P],
+    "optimi_b200_weight_gradient": [_P, _L, _P, _L, _P, _L, _P, _L, _L, _L, _I, _P, _P, _Z, _P],
+}
+SIGNATURES.update(ACTIVATION_SIGNATURES)
+EXPORTS = list(SIGNATURES) + ["optimi_b200_rms_norm_backward_workspace_bytes", "optimi_b200_weight_gradient_workspace_bytes"] + ["optimi_b200_push_begin", "optimi_b200_push_end", "optimi_b200_pull_begin", "optimi_b200_pull_end", "optimi_b200_last_error", "optimi_b200_version", "optimi_b200_launch_count", "optimi_b200_stableadamw_workspace_bytes",
                                    "optimi_b200_graph_record_begin", "optimi_b200_graph_record_end", "optimi_b200_graph_nodes_count",
                                    "optimi_b200_graph_nodes_free", "optimi_b200_graph_update_begin", "optimi_b200_graph_update_end",
                                    "optimi_b200_grad_scale_begin", "optimi_b200_grad_scale_end", "optimi_b200_grad_clip_workspace_bytes",
@@ -49,6 +59,10 @@ def _load() -> ctypes.CDLL:
         fn = getattr(lib, name)
         fn.argtypes = argtypes
         fn.restype = _I
+    lib.optimi_b200_rms_norm_backward_workspace_bytes.restype = _Z
+    lib.optimi_b200_rms_norm_backward_workspace_bytes.argtypes = [_L, _L]
+    lib.optimi_b200_weight_gradient_workspace_bytes.restype = _Z
+    lib.optimi_b200_weight_gradient_workspace_bytes.argtypes = [_L, _L, _L]
     lib.optimi_b200_last_error.restype = ctypes.c_char_p
     lib.optimi_b200_last_error.argtypes = []
     lib.optimi_b200_version.restype = _I

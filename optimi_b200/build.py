@@ -16,7 +16,9 @@ import sys
 
 PKG = os.path.dirname(os.path.abspath(__file__))
 SRC = os.path.join(PKG, "csrc", "optimi_b200.cu")
+ACTIVATION_SRCS = [os.path.join(PKG, "csrc", "activation_ops.cu"), os.path.join(PKG, "csrc", "weight_gradient.cu")]
 DEPS = [SRC, os.path.join(PKG, "csrc", "mta_common.cuh"), os.path.join(PKG, "csrc", "optimizer_ops.cuh"),
+        *ACTIVATION_SRCS, os.path.join(PKG, "csrc", "activation_common.cuh"),
         os.path.join(os.path.dirname(PKG), "include", "optimi_b200.h")]  # fmt: skip
 LIB_DIR = os.path.join(PKG, "lib")
 LIB = os.path.join(LIB_DIR, "liboptimi_b200.so")
@@ -53,7 +55,7 @@ def up_to_date() -> bool:
         return fh.read().strip() == source_hash()
 
 
-N_PARTS = 3  # the source compiles as independent translation units (OPTIMI_PART), built in parallel
+N_PARTS = 3  # the step source compiles as independent translation units (OPTIMI_PART), built in parallel
 
 
 def build(force: bool = False, verbose: bool = False) -> str:
@@ -75,10 +77,11 @@ def build(force: bool = False, verbose: bool = False) -> str:
         compile_flags = [f for f in NVCC_FLAGS if f not in ("-shared", "--use-local-env")]
         with tempfile.TemporaryDirectory(dir=LIB_DIR, prefix=".build-") as tmp:
             objs, procs = [], []
-            for part in range(N_PARTS):
-                obj = os.path.join(tmp, f"part{part}.o")
+            units = [(SRC, [f"-DOPTIMI_PART={part}"]) for part in range(N_PARTS)] + [(src, []) for src in ACTIVATION_SRCS]
+            for number, (src, defines) in enumerate(units):
+                obj = os.path.join(tmp, f"part{number}.o")
                 objs.append(obj)
-                cmd = [nvcc, *ccbin, *compile_flags, *(["-Xptxas", "-v"] if verbose else []), f"-DOPTIMI_PART={part}", "-c", "-o", obj, SRC]
+                cmd = [nvcc, *ccbin, *compile_flags, *(["-Xptxas", "-v"] if verbose else []), *defines, "-c", "-o", obj, src]
                 procs.append((cmd, subprocess.Popen(cmd, stdout=subprocess.PIPE, stderr=subprocess.PIPE, text=True)))
             log = ""
             for cmd, p in procs:
