@@ -213,16 +213,19 @@ def weight_gradient(grad: Tensor, saved: CompressedActivation) -> Tensor:
         raise RuntimeError(f"{name}: `saved` ({saved.dtype}, {saved.device}) does not match `grad` ({grad.dtype}, {grad.device})")
     if grad.dim() == 0 or _rows(grad.shape) != _rows(saved.shape):
         raise RuntimeError(f"{name}: `grad` {tuple(grad.shape)} and `saved` {tuple(saved.shape)} have different numbers of tokens")
-    m = _as_rows(grad)
+    m = _as_rows(grad.detach())
     rows, outputs = m.shape
     channels = saved.shape[-1]
+    if m.data_ptr() % 16 or rows > 1 and m.stride(0) % 8 or rows == 1 and outputs % 8:  # the copy engine loads from multiples of 16 bytes
+        m = torch.empty((rows, -(-outputs // 8) * 8), dtype=grad.dtype, device=grad.device)[:, :outputs].copy_(m)
+    stride = m.stride(0) if rows > 1 else -(-outputs // 8) * 8
     dw = torch.empty((outputs, channels), dtype=grad.dtype, device=grad.device)
     scale = None if saved.channel_scale is None else saved.channel_scale.detach().contiguous()
     need = _lib.LIB.optimi_b200_weight_gradient_workspace_bytes(rows, outputs, channels)
     workspace = torch.empty(need, dtype=torch.uint8, device=grad.device) if need else None
     with _on_device(grad.device):
         _lib.check(_lib.LIB.optimi_b200_weight_gradient(
-            m.data_ptr(), m.stride(0), saved.codes.data_ptr(), saved.codes.stride(0), saved.exponents.data_ptr(),
+            m.data_ptr(), stride, saved.codes.data_ptr(), saved.codes.stride(0), saved.exponents.data_ptr(),
             saved.exponents.stride(0), _ptr(scale), rows, outputs, channels, _lib.DTYPE_CODE[grad.dtype], dw.data_ptr(),
             _ptr(workspace), need, _stream(grad.device)))  # fmt: skip
     return dw

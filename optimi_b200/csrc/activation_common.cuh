@@ -18,6 +18,7 @@
 #include <atomic>
 #include <cstdarg>
 #include <cstdio>
+#include <type_traits>
 
 namespace optimi {
 

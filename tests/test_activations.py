@@ -97,10 +97,14 @@ def test_entry_points_reject_bad_arguments_without_launching():
     refused(L.optimi_b200_weight_gradient(*with_(dw, _11=None)), b"grad_weight is NULL")
     refused(L.optimi_b200_weight_gradient(*with_(dw, _0=None)), b"grad is NULL")
     refused(L.optimi_b200_weight_gradient(*with_(dw, _3=32)), b"pitch")
+    refused(L.optimi_b200_weight_gradient(*with_(dw, _0=ctypes.c_void_p(0x1008))), b"begin on 16 bytes")
+    refused(L.optimi_b200_weight_gradient(*with_(dw, _1=68)), b"begin on 16 bytes")
+    refused(L.optimi_b200_weight_gradient(*with_(dw, _1=56)), b"begin on 16 bytes")
+    refused(L.optimi_b200_weight_gradient_status(None), b"gave_up is NULL")
     # nothing to do is not an error
     assert L.optimi_b200_compress(None, 0, 0, 64, 1, None, 0, None, 0, None) == 0
     assert L.optimi_b200_rms_norm(*with_(norm, _5=0)) == 0
-    assert L.optimi_b200_weight_gradient(*with_(dw, _8=0)) == 0
+    assert L.optimi_b200_weight_gradient(*with_(dw, _9=0)) == 0
     assert L.optimi_b200_launch_count() == before
 
 

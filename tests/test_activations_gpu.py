@@ -424,6 +424,15 @@ def test_weight_gradient_keeps_nans_where_they_belong(dtype):
     assert torch.isfinite(dw[~bad]).all()
 
 
+def test_no_wait_ran_out():
+    import ctypes
+
+    from optimi_b200 import _lib
+
+    flag = ctypes.c_int(-1)
+    assert _lib.LIB.optimi_b200_weight_gradient_status(ctypes.byref(flag)) == 0 and flag.value == 0
+
+
 def test_weight_gradient_same_bits_every_time():
     a = act()
     x, grad = loud((5000, 320), torch.bfloat16, 1).cuda(), normal((5000, 200), torch.bfloat16, 2).cuda()
