@@ -14,12 +14,17 @@
 namespace optimi {
 namespace act {
 
-constexpr int kM = 128, kN = 256, kK = 64;           // channels, outputs, tokens of a block
-constexpr int kStages = 5;
-constexpr int kGradBytes = kK * kN * 2, kCodeBytes = kK * kM, kStageBytes = kGradBytes + kCodeBytes;
+// A pair of blocks on two neighbouring SMs works on one tile of 256 channels x 256 outputs, 64 tokens at a time.  Each holds
+// the codes, X^T and the results of its 128 channels, and the gradients of its 128 outputs; the instruction reads the other
+// half of the gradients from the partner's shared memory.
+constexpr int kM = 128, kN = 256, kK = 64;           // channels of a block, outputs of the pair, tokens of a step
+constexpr int kStages = 8;
+constexpr int kGradBytes = kK * (kN / 2) * 2, kCodeBytes = kK * kM, kStageBytes = kGradBytes + kCodeBytes;
 constexpr int kSmemBytes = kStages * kStageBytes + 1024;
 constexpr int kAColumns = kK / 2;                    // 32-bit columns of tensor memory of one block of X^T
-constexpr int kThreads = 192;                        // four warps that convert and write results, one that loads, one that multiplies
+constexpr int kMakers = 8;                           // warps that convert, in two sets that take turns, and write results
+constexpr int kLoader = kMakers, kIssuer = kMakers + 1;
+constexpr int kThreads = 32 * (kMakers + 2);
 constexpr int kWaitLimit = 1 << 22;                  // polls after which a wait gives up
 
 // Set by a kernel whose wait gave up (its results are NaN); read by optimi_b200_weight_gradient_status.
@@ -30,8 +35,16 @@ static __device__ __forceinline__ uint32_t smem_of(const void* p) { return (uint
 static __device__ __forceinline__ void barrier_init(uint32_t bar, uint32_t count) {
   asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count));
 }
-static __device__ __forceinline__ void barrier_arrive(uint32_t bar) {
-  asm volatile("mbarrier.arrive.release.cta.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
+// The same barrier of the pair's first block.
+static __device__ __forceinline__ uint32_t in_first(uint32_t bar) {
+  uint32_t at;
+  asm("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(at) : "r"(bar));
+  return at;
+}
+// Relaxed: what it announces lies in tensor memory, which tcgen05.wait::st and the fences around the barrier order; a release
+// over the cluster would wait for the loads under way too (measured: half the kernel's time).
+static __device__ __forceinline__ void barrier_arrive(uint32_t remote) {
+  asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(remote) : "memory");
 }
 static __device__ __forceinline__ void barrier_expect(uint32_t bar, uint32_t bytes) {
   asm volatile("mbarrier.arrive.expect_tx.release.cta.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
@@ -50,8 +63,18 @@ static __device__ __forceinline__ bool barrier_wait(uint32_t bar, uint32_t parit
   return false;
 }
 
+static __device__ __forceinline__ void pair_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// The barrier is arrived at in both blocks once all the multiplications issued so far are done.
+static __device__ __forceinline__ void commit_to_pair(uint32_t bar) {
+  asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar), "h"((uint16_t)3)
+               : "memory");
+}
+
+// `bar` may be a barrier of either block of the pair.
 static __device__ __forceinline__ void load_tile(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
-  asm volatile("cp.async.bulk.tensor.2d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
+  asm volatile("cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
                "l"(map), "r"(x), "r"(y), "r"(bar)
                : "memory");
 }
@@ -62,11 +85,11 @@ static __device__ __forceinline__ uint64_t grad_descriptor(uint32_t addr) {
   return (uint64_t)((addr & 0x3ffff) >> 4) | (uint64_t)(kK * 128 >> 4) << 16 | (uint64_t)(1024 >> 4) << 32 | 1ull << 46 | 2ull << 61;
 }
 
-// D in fp32; A and B in T; A as it lies in tensor memory, B transposed (its outputs are contiguous); N and M.
+// D in fp32; A and B in T; A as it lies in tensor memory, B transposed (its outputs are contiguous); N and M of the pair.
 template <typename T>
 static __device__ __forceinline__ constexpr uint32_t instruction_descriptor() {
   constexpr uint32_t kind = sizeof(T) == 2 && !std::is_same<T, __half>::value ? 1 : 0;
-  return 1u << 4 | kind << 7 | kind << 10 | 1u << 16 | (uint32_t)(kN >> 3) << 17 | (uint32_t)(kM >> 4) << 24;
+  return 1u << 4 | kind << 7 | kind << 10 | 1u << 16 | (uint32_t)(kN >> 3) << 17 | (uint32_t)(2 * kM >> 4) << 24;
 }
 
 // 2^(e - 127) for two exponent bytes, as a pair of T.  bf16: the byte is the exponent field (255 gives an infinity, which
@@ -101,61 +124,72 @@ template <> __device__ __forceinline__ uint32_t code_pair<__half>(uint32_t codes
 }
 
 template <typename T>
-__global__ void __launch_bounds__(kThreads, 1)
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     weight_gradient_kernel(const __grid_constant__ CUtensorMap grad_map, const __grid_constant__ CUtensorMap code_map,
                            const uint8_t* __restrict__ exponents, int64_t epitch, const T* __restrict__ channel_scale, int rows,
                            int outputs, int channels, T* __restrict__ dw) {
   extern __shared__ uint8_t dynamic[];
-  __shared__ __align__(8) uint64_t bars[3 * kStages + 1];
-  __shared__ __align__(4) uint8_t bytes[4][2][kK];
+  __shared__ __align__(8) uint64_t bars[4 * kStages + 1];
+  __shared__ __align__(4) uint8_t bytes[kMakers][2][kK];
   __shared__ uint32_t tmem_base;
   __shared__ int gave_up;
   const uint32_t tiles = (smem_of(dynamic) + 1023) & ~1023u;
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-  const uint32_t full = smem_of(bars), made = full + 8 * kStages, empty = made + 8 * kStages, done = empty + 8 * kStages;
+  const int half = blockIdx.x % 2;  // which block of the pair
+  // codes: this block's codes are there.  grads, made (the first block's): both blocks' gradients, both halves of X^T are there.
+  // empty: the multiplications that read a stage are done.
+  const uint32_t codes_in = smem_of(bars), grads_in = codes_in + 8 * kStages, made = grads_in + 8 * kStages, empty = made + 8 * kStages,
+                 done = empty + 8 * kStages;
   const int c0 = blockIdx.x * kM, o0 = blockIdx.y * kN;
   const int blocks = (rows + kK - 1) / kK;
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < kStages; s++) {
-      barrier_init(full + 8 * s, 1);
-      barrier_init(made + 8 * s, 4);
+      barrier_init(codes_in + 8 * s, 1);
+      barrier_init(grads_in + 8 * s, 1);
+      barrier_init(made + 8 * s, 2 * 4);  // four warps of each block
       barrier_init(empty + 8 * s, 1);
     }
     barrier_init(done, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     gave_up = 0;
   }
-  if (warp == 5) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_of(&tmem_base)) : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+  if (warp == kIssuer) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_of(&tmem_base)) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
   }
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   __syncthreads();
+  pair_sync();
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
   const uint32_t tmem = tmem_base, tmem_a = tmem + kN;
   bool ok = true;
 
-  if (warp == 4) {
+  if (warp == kLoader) {
     if (lane == 0) {
       int b = 0;
       for (; b < blocks; b++) {
         const int s = b % kStages;
         if (b >= kStages && !barrier_wait(empty + 8 * s, (b / kStages - 1) & 1)) break;
-        const uint32_t at = tiles + s * kStageBytes, bar = full + 8 * s;
-        barrier_expect(bar, kStageBytes);
-        for (int j = 0; j < kN / 64; j++) load_tile(at + j * kK * 128, &grad_map, o0 + j * 64, b * kK, bar);
-        load_tile(at + kGradBytes, &code_map, c0, b * kK, bar);
+        const uint32_t at = tiles + s * kStageBytes, grads = in_first(grads_in + 8 * s);
+        barrier_expect(codes_in + 8 * s, kCodeBytes);
+        load_tile(at + kGradBytes, &code_map, c0, b * kK, codes_in + 8 * s);
+        if (half == 0) barrier_expect(grads_in + 8 * s, 2 * kGradBytes);
+        for (int j = 0; j < kN / 2 / 64; j++) load_tile(at + j * kK * 128, &grad_map, o0 + half * (kN / 2) + j * 64, b * kK, grads);
       }
       ok = b == blocks;
-      // nothing of this block's shared memory is given back while a copy into it is under way
-      for (int n = b > kStages ? b - kStages : 0; n < b; n++) ok &= barrier_wait(full + 8 * (n % kStages), (n / kStages) & 1);
+      // Nothing of a block's shared memory is given back while a copy into it is under way: both blocks wait for the codes they
+      // asked for, the first for the gradients of both.  (The partner stays until the first block is here too.)
+      for (int n = b > kStages ? b - kStages : 0; n < b; n++) {
+        ok &= barrier_wait(codes_in + 8 * (n % kStages), (n / kStages) & 1);
+        if (half == 0) ok &= barrier_wait(grads_in + 8 * (n % kStages), (n / kStages) & 1);
+      }
     }
-  } else if (warp == 5) {
-    if (lane == 0) {
-      for (int b = 0; b < blocks && ok; b++) {
-        const int s = b % kStages, parity = (b / kStages) & 1;
-        ok = barrier_wait(full + 8 * s, parity) && barrier_wait(made + 8 * s, parity);
+  } else if (warp == kIssuer) {
+    if (lane == 0 && half == 0) {
+      for (int b = 0; b < blocks; b++) {
+        const int s = b % kStages;
+        ok = barrier_wait(grads_in + 8 * s, (b / kStages) & 1) && barrier_wait(made + 8 * s, (b / kStages) & 1);
         if (!ok) break;
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         const uint64_t desc = grad_descriptor(tiles + s * kStageBytes);
@@ -164,34 +198,36 @@ __global__ void __launch_bounds__(kThreads, 1)
           const uint32_t accumulate = b > 0 || k > 0;
           asm volatile(
               "{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\n"
-              "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}" ::"r"(tmem),
+              "tcgen05.mma.cta_group::2.kind::f16 [%0], [%1], %2, %3, p;\n}" ::"r"(tmem),
               "r"(tmem_a + s * kAColumns + k * 8), "l"(desc + (uint64_t)(k * 2048 >> 4)), "r"(instruction_descriptor<T>()), "r"(accumulate)
               : "memory");
         }
-        asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(empty + 8 * s) : "memory");
+        commit_to_pair(empty + 8 * s);
       }
-      asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(done) : "memory");
+      commit_to_pair(done);
     }
   } else {
-    // channels 32 * warp .. + 31 are this warp's rows of tensor memory, and one group of the format
-    const int group = c0 / kGroup + warp, quad = lane % 4;
+    // channels 32 * (warp % 4) .. + 31 of the block are this warp's rows of tensor memory, and one group of the format
+    const int part = warp % 4, set = warp / 4;
+    const int group = c0 / kGroup + part, quad = lane % 4;
     const bool live = group * kGroup < channels;
     const auto exponent = [&](int t) -> uint32_t { return live && t < rows ? exponents[(int64_t)t * epitch + group] : 0; };
-    uint32_t e0 = exponent(lane), e1 = exponent(lane + 32);
-    for (int b = 0; b < blocks && ok; b++) {
+    uint32_t e0 = exponent(set * kK + lane), e1 = exponent(set * kK + lane + 32);
+    for (int b = set; b < blocks; b += kMakers / 4) {
       const int s = b % kStages, parity = (b / kStages) & 1;
-      uint8_t* mine = bytes[warp][b & 1];
+      uint8_t* mine = bytes[warp][b / (kMakers / 4) & 1];
       mine[lane] = (uint8_t)e0, mine[lane + 32] = (uint8_t)e1;
       __syncwarp();
-      e0 = exponent((b + 1) * kK + lane), e1 = exponent((b + 1) * kK + lane + 32);
-      ok = barrier_wait(full + 8 * s, parity);
+      const int next = (b + kMakers / 4) * kK + lane;
+      e0 = exponent(next), e1 = exponent(next + 32);
+      ok = barrier_wait(codes_in + 8 * s, parity);
       if (!ok) break;
       const uint32_t codes = tiles + s * kStageBytes + kGradBytes;
       uint32_t low[16], high[16];
 #pragma unroll
       for (int j = 0; j < kK / 16; j++) {
-        // a 16 x 16 byte transpose each: thread l gets channel l / 4 (and + 8), tokens 4 * (l % 4) .. + 3
-        const int t = j * 16 + lane % 16, chunk = 2 * warp + lane / 16;
+        // two 16 x 16 byte transposes: thread l gets channel l / 4 (and + 8), tokens 4 * (l % 4) .. + 3 of each
+        const int t = j * 16 + lane % 16, chunk = 2 * part + lane / 16;
         uint32_t r[4];
         asm volatile("ldmatrix.sync.aligned.m16n16.x2.trans.shared.b8 {%0, %1, %2, %3}, [%4];"
                      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
@@ -204,7 +240,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           high[4 * j + 2 * i] = code_pair<T>(r[2 + i], 0x4140, s01), high[4 * j + 2 * i + 1] = code_pair<T>(r[2 + i], 0x4342, s23);
         }
       }
-      const uint32_t to = tmem_a + s * kAColumns + ((uint32_t)(warp * 32) << 16);
+      const uint32_t to = tmem_a + s * kAColumns + ((uint32_t)(part * 32) << 16);
 #define STORE16(addr, v)                                                                                                            \
   asm volatile("tcgen05.st.sync.aligned.16x256b.x4.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" \
                ::"r"(addr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]),       \
@@ -216,7 +252,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
       asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
       __syncwarp();
-      if (lane == 0) barrier_arrive(made + 8 * s);
+      if (lane == 0) barrier_arrive(in_first(made + 8 * s));
     }
     ok = barrier_wait(done, 0) && ok;
   }
@@ -225,32 +261,33 @@ __global__ void __launch_bounds__(kThreads, 1)
   __syncthreads();
   if (gave_up && threadIdx.x == 0) g_gave_up = 1;
 
-  if (warp < 4) {
+  if (warp < kMakers) {
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-    const int c = c0 + warp * 32 + lane;
+    const int part = warp % 4;
+    const int c = c0 + part * 32 + lane;
     const float scale = channel_scale && c < channels ? to_f32(channel_scale[c]) : 1.0f;
     const bool lost = gave_up;
-    for (int n = 0; n < kN && o0 + n < outputs; n += 16) {
+    const int first = warp / 4 * (kN / (kMakers / 4));
+    for (int n = first; n < first + kN / (kMakers / 4) && o0 + n < outputs; n += 16) {
       uint32_t v[16];
       asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
                    : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]), "=r"(v[9]),
                      "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
-                   : "r"(tmem + n + ((uint32_t)(warp * 32) << 16)));
+                   : "r"(tmem + n + ((uint32_t)(part * 32) << 16)));
       asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 #pragma unroll
       for (int i = 0; i < 16; i++) {
-        const float d = blocks == 0 ? 0.0f : lost ? __int_as_float(0x7fffffff) : __uint_as_float(v[i]);
+        const float d = lost ? __int_as_float(0x7fffffff) : __uint_as_float(v[i]);
         if (o0 + n + i < outputs && c < channels) dw[(int64_t)(o0 + n + i) * channels + c] = from_f32<T>(__fmul_rn(d, scale));
       }
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   }
   __syncwarp();
-  __syncthreads();
-  if (warp == 5) {
-    __syncwarp();
+  pair_sync();  // the partner may still read this block's gradients or arrive at its barriers
+  if (warp == kIssuer) {
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, 512;" ::"r"(tmem));
   }
 }
 
@@ -289,7 +326,7 @@ static int launch_weight_gradient(const char* fn, const CUtensorMap& grad_map, c
                                   int64_t epitch, const void* channel_scale, int rows, int outputs, int channels, void* dw, cudaStream_t s) {
   cudaError_t e = cudaFuncSetAttribute(weight_gradient_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes);
   if (e != cudaSuccess) return fail(OPTIMI_ERR_CUDA, "%s: %s", fn, cudaGetErrorString(e));
-  const dim3 grid((channels + kM - 1) / kM, (outputs + kN - 1) / kN);
+  const dim3 grid((channels + 2 * kM - 1) / (2 * kM) * 2, (outputs + kN - 1) / kN);
   weight_gradient_kernel<T><<<grid, kThreads, kSmemBytes, s>>>(grad_map, code_map, (const uint8_t*)exponents, epitch,
                                                               (const T*)channel_scale, rows, outputs, channels, (T*)dw);
   return launched(fn);
