@@ -115,5 +115,172 @@ static __device__ __forceinline__ int encode(double x, int e) {
   return __double2int_rn(fmin(fmax(x * (double)power_of(254 - e), -127.0), 127.0));
 }
 
+// ---------------------------------------------------------------------------------------------
+// chunks: C neighbouring values of a row in one thread, 16 bytes where rows begin on 16 bytes, else one value
+// ---------------------------------------------------------------------------------------------
+template <typename T, int C>
+struct Chunk {
+  static constexpr int kWords = C * (int)sizeof(T) >= 4 ? C * (int)sizeof(T) / 4 : 1;
+  static constexpr int kLanes = kGroup / C;  // neighbouring lanes that hold a group
+  uint32_t w[kWords];
+
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int i = 0; i < kWords; i++) w[i] = 0;
+  }
+  __device__ __forceinline__ void load(const T* p) {
+    if constexpr (kWords == 4) {
+      const uint4 v = *reinterpret_cast<const uint4*>(p);
+      w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
+    } else if constexpr (sizeof(T) == 4) {
+      w[0] = __float_as_uint(*p);
+    } else {
+      w[0] = *reinterpret_cast<const unsigned short*>(p);
+    }
+  }
+  __device__ __forceinline__ void store(T* p) const {
+    if constexpr (kWords == 4) *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+    else if constexpr (sizeof(T) == 4) *p = __uint_as_float(w[0]);
+    else *reinterpret_cast<unsigned short*>(p) = (unsigned short)w[0];
+  }
+  __device__ __forceinline__ float get(int i) const {
+    if constexpr (sizeof(T) == 4) return __uint_as_float(w[i]);
+    else if constexpr (std::is_same<T, __half>::value) return __half2float(__ushort_as_half((unsigned short)(w[i / 2] >> (i % 2 * 16))));
+    else return __uint_as_float(i % 2 ? w[i / 2] & 0xffff0000u : w[i / 2] << 16);
+  }
+  // v[0..C-1], rounded to T
+  __device__ __forceinline__ void set(const float* v) {
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+      for (int i = 0; i < C; i++) w[i] = __float_as_uint(v[i]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < kWords; i++) {
+        const float high = C == 1 ? 0.0f : v[C == 1 ? 0 : 2 * i + 1];
+        if constexpr (std::is_same<T, __half>::value) asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(w[i]) : "f"(high), "f"(v[C == 1 ? 0 : 2 * i]));
+        else asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(w[i]) : "f"(high), "f"(v[C == 1 ? 0 : 2 * i]));
+      }
+    }
+  }
+  // The largest magnitude, as fp32 bits: magnitudes compare as whole numbers, NaNs above infinity.
+  __device__ __forceinline__ uint32_t amax() const {
+    if constexpr (sizeof(T) == 4) {
+      uint32_t m = 0;
+#pragma unroll
+      for (int i = 0; i < kWords; i++) m = max(m, w[i] & 0x7fffffffu);
+      return m;
+    } else {
+      uint32_t m = 0;
+#pragma unroll
+      for (int i = 0; i < kWords; i++) m = __vmaxu2(m, w[i] & 0x7fff7fffu);
+      m = max(m & 0xffffu, m >> 16);
+      if constexpr (std::is_same<T, __half>::value) return __float_as_uint(__half2float(__ushort_as_half((unsigned short)m)));
+      else return m << 16;
+    }
+  }
+};
+
+// The largest of a group's magnitudes, in all its lanes.
+template <int kLanes>
+static __device__ __forceinline__ uint32_t group_max(uint32_t m) {
+  if constexpr (kLanes == 32) return __reduce_max_sync(~0u, m);
+#pragma unroll
+  for (int d = 1; d < kLanes; d *= 2) m = max(m, __shfl_xor_sync(~0u, m, d));
+  return m;
+}
+
+// C codes, in bytes.
+template <int C>
+struct CodeChunk {
+  static constexpr int kWords = C >= 4 ? C / 4 : 1;
+  uint32_t w[kWords];
+
+  // From values in fp32 that are at most 127.5 in a unit of 2^(e - 127), or more where e was held at its largest.  One fused
+  // multiply-add gives product, rounding and code: the product is exact, and the sum with 1.5 * 2^23 rounds to a whole number.
+  template <typename T>
+  __device__ __forceinline__ void encode(const float* v, int e) {
+    const float inverse = power_of(254 - e);
+    uint32_t c[C];
+    if (e >= Range<T>::high) {  // the top of the range, or a NaN group: rare
+#pragma unroll
+      for (int i = 0; i < C; i++) c[i] = (uint32_t)act::encode(v[i], e);
+    } else {
+#pragma unroll
+      for (int i = 0; i < C; i++) c[i] = __float_as_uint(__fmaf_rn(v[i], inverse, kToInt));
+    }
+    set(c);
+  }
+  template <typename T>
+  __device__ __forceinline__ void encode(const double* v, int e) {
+    uint32_t c[C];
+#pragma unroll
+    for (int i = 0; i < C; i++) c[i] = (uint32_t)act::encode(v[i], e);
+    set(c);
+  }
+  __device__ __forceinline__ void set(const uint32_t* c) {
+    if constexpr (C == 1) {
+      w[0] = c[0];
+    } else {
+#pragma unroll
+      for (int i = 0; i < kWords; i++)
+        w[i] = __byte_perm(__byte_perm(c[4 * i], c[4 * i + 1], 0x0040), __byte_perm(c[4 * i + 2], c[4 * i + 3], 0x0040), 0x5410);
+    }
+  }
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int i = 0; i < kWords; i++) w[i] = 0;
+  }
+  __device__ __forceinline__ void load(const int8_t* p) {
+    if constexpr (C == 8) {
+      const uint2 v = *reinterpret_cast<const uint2*>(p);
+      w[0] = v.x, w[1] = v.y;
+    } else if constexpr (C == 4) {
+      w[0] = *reinterpret_cast<const uint32_t*>(p);
+    } else {
+      w[0] = *reinterpret_cast<const uint8_t*>(p);
+    }
+  }
+  __device__ __forceinline__ void store(int8_t* p) const {
+    if constexpr (C == 8) *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
+    else if constexpr (C == 4) *reinterpret_cast<uint32_t*>(p) = w[0];
+    else *p = (int8_t)w[0];
+  }
+  // Code i as fp32: the byte with its sign bit flipped, set into the low bits of 2^23, is 2^23 + 128 + code.
+  __device__ __forceinline__ float get(int i) const {
+    return __uint_as_float(__byte_perm(w[i / 4] ^ 0x80808080u, 0x4b000000u, 0x7440 + i % 4)) - 8388736.0f;
+  }
+};
+
+// 2^(e - 127) for two exponent bytes, as a pair of T.  bf16: the byte is the exponent field (255 gives an infinity, which
+// makes the zero codes of its group NaN).  fp16: through fp32, exact down to the subnormal 2^-24.
+template <typename T> static __device__ __forceinline__ uint32_t scale_pair(uint32_t bytes, uint32_t select);
+template <> __device__ __forceinline__ uint32_t scale_pair<__nv_bfloat16>(uint32_t bytes, uint32_t select) {
+  return __byte_perm(bytes, 0, select) << 7;
+}
+template <> __device__ __forceinline__ uint32_t scale_pair<__half>(uint32_t bytes, uint32_t select) {
+  const uint32_t p = __byte_perm(bytes, 0, select);
+  uint32_t r;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(__uint_as_float((p >> 16) << 23)), "f"(__uint_as_float((p & 0xff) << 23)));
+  return r;
+}
+
+// Two codes (bytes picked by `select`) times two scales, exactly.  A byte set into the low mantissa bits of a constant is a
+// whole number plus that constant, which a subtraction takes off again.
+// bf16 has 7 such bits: 0x43 << 8 is 128, so the low 7 bits give 128 + b & 127 and the sign bit, in the exponent, tells 128 from 256.
+template <typename T> static __device__ __forceinline__ uint32_t code_pair(uint32_t codes, uint32_t select, uint32_t scale);
+template <> __device__ __forceinline__ uint32_t code_pair<__nv_bfloat16>(uint32_t codes, uint32_t select, uint32_t scale) {
+  const uint32_t p = __byte_perm(codes, 0x43, select), with = p & 0xff7fff7fu, without = p & 0xff80ff80u;
+  uint32_t r;
+  asm("{\n.reg .b32 t;\nsub.rn.bf16x2 t, %1, %2;\nmul.rn.bf16x2 %0, t, %3;\n}" : "=r"(r) : "r"(with), "r"(without), "r"(scale));
+  return r;
+}
+// fp16 has 10: 0x64 << 8 is 1024, and the byte with its sign bit flipped is code + 128.
+template <> __device__ __forceinline__ uint32_t code_pair<__half>(uint32_t codes, uint32_t select, uint32_t scale) {
+  const uint32_t p = __byte_perm(codes ^ 0x80808080u, 0x64, select);
+  uint32_t r;
+  asm("{\n.reg .b32 t;\nsub.rn.f16x2 t, %1, %2;\nmul.rn.f16x2 %0, t, %3;\n}" : "=r"(r) : "r"(p), "r"(0x64806480u), "r"(scale));
+  return r;
+}
+
 }  // namespace act
 }  // namespace optimi

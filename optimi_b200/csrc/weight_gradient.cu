@@ -92,37 +92,6 @@ static __device__ __forceinline__ constexpr uint32_t instruction_descriptor() {
   return 1u << 4 | kind << 7 | kind << 10 | 1u << 16 | (uint32_t)(kN >> 3) << 17 | (uint32_t)(2 * kM >> 4) << 24;
 }
 
-// 2^(e - 127) for two exponent bytes, as a pair of T.  bf16: the byte is the exponent field (255 gives an infinity, which
-// makes the zero codes of its group NaN).  fp16: through fp32, exact down to the subnormal 2^-24.
-template <typename T> static __device__ __forceinline__ uint32_t scale_pair(uint32_t bytes, uint32_t select);
-template <> __device__ __forceinline__ uint32_t scale_pair<__nv_bfloat16>(uint32_t bytes, uint32_t select) {
-  return __byte_perm(bytes, 0, select) << 7;
-}
-template <> __device__ __forceinline__ uint32_t scale_pair<__half>(uint32_t bytes, uint32_t select) {
-  const uint32_t p = __byte_perm(bytes, 0, select);
-  uint32_t r;
-  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(__uint_as_float((p >> 16) << 23)), "f"(__uint_as_float((p & 0xff) << 23)));
-  return r;
-}
-
-// Two codes (bytes picked by `select`) times two scales, exactly.  A byte set into the low mantissa bits of a constant is a
-// whole number plus that constant, which a subtraction takes off again.
-// bf16 has 7 such bits: 0x43 << 8 is 128, so the low 7 bits give 128 + b & 127 and the sign bit, in the exponent, tells 128 from 256.
-template <typename T> static __device__ __forceinline__ uint32_t code_pair(uint32_t codes, uint32_t select, uint32_t scale);
-template <> __device__ __forceinline__ uint32_t code_pair<__nv_bfloat16>(uint32_t codes, uint32_t select, uint32_t scale) {
-  const uint32_t p = __byte_perm(codes, 0x43, select), with = p & 0xff7fff7fu, without = p & 0xff80ff80u;
-  uint32_t r;
-  asm("{\n.reg .b32 t;\nsub.rn.bf16x2 t, %1, %2;\nmul.rn.bf16x2 %0, t, %3;\n}" : "=r"(r) : "r"(with), "r"(without), "r"(scale));
-  return r;
-}
-// fp16 has 10: 0x64 << 8 is 1024, and the byte with its sign bit flipped is code + 128.
-template <> __device__ __forceinline__ uint32_t code_pair<__half>(uint32_t codes, uint32_t select, uint32_t scale) {
-  const uint32_t p = __byte_perm(codes ^ 0x80808080u, 0x64, select);
-  uint32_t r;
-  asm("{\n.reg .b32 t;\nsub.rn.f16x2 t, %1, %2;\nmul.rn.f16x2 %0, t, %3;\n}" : "=r"(r) : "r"(p), "r"(0x64806480u), "r"(scale));
-  return r;
-}
-
 template <typename T>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     weight_gradient_kernel(const __grid_constant__ CUtensorMap grad_map, const __grid_constant__ CUtensorMap code_map,
