@@ -20,14 +20,14 @@ activation in place of the original.  CUDA tensors only, like the optimizers.
 
 from __future__ import annotations
 
-from typing import Any, Callable, NamedTuple
+from collections.abc import Callable, Sequence
+from typing import Any, NamedTuple
 from warnings import warn
 
 import torch
 import torch.nn.functional as F
 import torch.utils.checkpoint
 from torch import Tensor, nn
-from torch.autograd.function import once_differentiable
 
 from . import _lib
 
@@ -50,7 +50,7 @@ class CompressedActivation:
     NaN and reads back as NaNs.  `channel_scale`, where given, multiplies the last dimension (a norm's weight).
     """
 
-    __slots__ = ("codes", "exponents", "shape", "dtype", "channel_scale")
+    __slots__ = ("_codes", "_exponents", "_buffer", "shape", "dtype", "channel_scale")
 
     def __init__(self, codes: Tensor, exponents: Tensor, shape, dtype: torch.dtype, channel_scale: Tensor | None = None):
         shape = torch.Size(shape)
@@ -74,22 +74,51 @@ class CompressedActivation:
                 raise ValueError("rows of codes and exponents must not overlap")
         if channel_scale is not None and (channel_scale.shape != shape[-1:] or channel_scale.dtype != dtype or channel_scale.device != codes.device):
             raise ValueError(f"channel_scale must be a {dtype} tensor of {cols} values on {codes.device}")
-        self.codes, self.exponents, self.shape, self.dtype, self.channel_scale = codes, exponents, shape, dtype, channel_scale
+        self._codes, self._exponents, self._buffer = codes, exponents, None
+        self.shape, self.dtype, self.channel_scale = shape, dtype, channel_scale
 
     @classmethod
-    def _of(cls, codes, exponents, shape, dtype, channel_scale=None) -> CompressedActivation:
-        """For buffers this module made itself: no checks."""
+    def _of(cls, tensors: Sequence[Tensor], shape, dtype, channel_scale=None) -> CompressedActivation:
+        """From what `_tensors` gave, or one buffer of `_buffer_bytes` that holds the codes, then the exponents; no checks."""
         self = object.__new__(cls)
-        self.codes, self.exponents, self.shape, self.dtype, self.channel_scale = codes, exponents, shape, dtype, channel_scale
+        self._codes, self._exponents, self._buffer = (*tensors, None) if len(tensors) == 2 else (None, None, tensors[0])
+        self.shape, self.dtype, self.channel_scale = shape, dtype, channel_scale
         return self
+
+    def _tensors(self) -> tuple[Tensor, ...]:
+        """What holds the codes and exponents, to be kept with `ctx.save_for_backward`."""
+        return (self._codes, self._exponents) if self._buffer is None else (self._buffer,)
+
+    def _layout(self) -> tuple[int, int, int, int]:
+        """Addresses and pitches of codes and exponents."""
+        if self._buffer is None:
+            c, e = self._codes, self._exponents
+            return c.data_ptr(), c.stride(0), e.data_ptr(), e.stride(0)
+        rows, groups = _rows(self.shape), -(-self.shape[-1] // GROUP)
+        at = self._buffer.data_ptr()
+        return at, groups * GROUP, at + rows * groups * GROUP, groups
+
+    @property
+    def codes(self) -> Tensor:
+        if self._buffer is None:
+            return self._codes
+        rows, groups = _rows(self.shape), -(-self.shape[-1] // GROUP)
+        return self._buffer[: rows * groups * GROUP].view(torch.int8).view(rows, groups * GROUP)
+
+    @property
+    def exponents(self) -> Tensor:
+        if self._buffer is None:
+            return self._exponents
+        rows, groups = _rows(self.shape), -(-self.shape[-1] // GROUP)
+        return self._buffer[rows * groups * GROUP : rows * groups * (GROUP + 1)].view(rows, groups)
 
     @property
     def device(self) -> torch.device:
-        return self.codes.device
+        return (self._codes if self._buffer is None else self._buffer).device
 
     @property
     def nbytes(self) -> int:
-        """Bytes of device memory the codes and exponents take."""
+        """Bytes of the codes and exponents."""
         return self.codes.numel() + self.exponents.numel()
 
     def decompress(self) -> Tensor:
@@ -145,7 +174,8 @@ def _ptr(t: Tensor | None) -> int | None:
 
 
 def _stream(device: torch.device) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
+    # torch.cuda.current_stream(device).cuda_stream without the Stream object around it (2 us of a 15 us call)
+    return torch._C._cuda_getCurrentRawStream(device.index)
 
 
 class _on_device:
@@ -165,10 +195,10 @@ class _on_device:
             self.guard.__exit__(*exc)
 
 
-def _new_codes(rows: int, cols: int, device: torch.device) -> tuple[Tensor, Tensor]:
-    groups = -(-cols // GROUP)
-    return (torch.empty((rows, groups * GROUP), dtype=torch.int8, device=device),
-            torch.empty((rows, groups), dtype=torch.uint8, device=device))  # fmt: skip
+def _buffer_bytes(rows: int, cols: int) -> tuple[int, int]:
+    """Bytes of codes and exponents in one buffer, and where 4-byte values may follow them."""
+    n = rows * -(-cols // GROUP) * (GROUP + 1)
+    return n, -(-n // 16) * 16
 
 
 def compress(x: Tensor) -> CompressedActivation:
@@ -178,24 +208,25 @@ def compress(x: Tensor) -> CompressedActivation:
         raise RuntimeError("compress: `x` must have at least one dimension")
     m = _as_rows(x)
     rows, cols = m.shape
-    codes, exponents = _new_codes(rows, cols, x.device)
-    with _on_device(x.device):
+    device = x.device
+    saved = CompressedActivation._of((torch.empty(_buffer_bytes(rows, cols)[0], dtype=torch.uint8, device=device),), x.shape, x.dtype)
+    with _on_device(device):
         _lib.check(_lib.LIB.optimi_b200_compress(
-            m.data_ptr(), m.stride(0), rows, cols, _lib.DTYPE_CODE[x.dtype], codes.data_ptr(), codes.stride(0),
-            exponents.data_ptr(), exponents.stride(0), _stream(x.device)))  # fmt: skip
-    return CompressedActivation._of(codes, exponents, x.shape, x.dtype)
+            m.data_ptr(), m.stride(0), rows, cols, _lib.DTYPE_CODE[x.dtype], *saved._layout(), _stream(device)))  # fmt: skip
+    return saved
 
 
 def decompress(saved: CompressedActivation) -> Tensor:
     """The activation `saved` stands for, its `channel_scale` applied."""
-    if saved.device.type != "cuda":
-        raise RuntimeError(f"decompress: `saved` lives on {saved.device}; optimi_b200 takes CUDA tensors only (there is no CPU path)")
-    out = torch.empty(saved.shape, dtype=saved.dtype, device=saved.device)
+    device = saved.device
+    if device.type != "cuda":
+        raise RuntimeError(f"decompress: `saved` lives on {device}; optimi_b200 takes CUDA tensors only (there is no CPU path)")
+    out = torch.empty(saved.shape, dtype=saved.dtype, device=device)
     scale = None if saved.channel_scale is None else saved.channel_scale.detach().contiguous()
-    with _on_device(saved.device):
+    with _on_device(device):
         _lib.check(_lib.LIB.optimi_b200_decompress(
-            saved.codes.data_ptr(), saved.codes.stride(0), saved.exponents.data_ptr(), saved.exponents.stride(0), _ptr(scale),
-            _rows(saved.shape), saved.shape[-1], _lib.DTYPE_CODE[saved.dtype], out.data_ptr(), _stream(saved.device)))  # fmt: skip
+            *saved._layout(), _ptr(scale), _rows(saved.shape), saved.shape[-1], _lib.DTYPE_CODE[saved.dtype], out.data_ptr(),
+            _stream(device)))  # fmt: skip
     return out
 
 
@@ -225,62 +256,71 @@ def weight_gradient(grad: Tensor, saved: CompressedActivation) -> Tensor:
     workspace = torch.empty(need, dtype=torch.uint8, device=grad.device) if need else None
     with _on_device(grad.device):
         _lib.check(_lib.LIB.optimi_b200_weight_gradient(
-            m.data_ptr(), stride, saved.codes.data_ptr(), saved.codes.stride(0), saved.exponents.data_ptr(),
-            saved.exponents.stride(0), _ptr(scale), rows, outputs, channels, _lib.DTYPE_CODE[grad.dtype], dw.data_ptr(),
+            m.data_ptr(), stride, *saved._layout(), _ptr(scale), rows, outputs, channels, _lib.DTYPE_CODE[grad.dtype], dw.data_ptr(),
             _ptr(workspace), need, _stream(grad.device)))  # fmt: skip
     return dw
 
 
 def _norm_forward(x: Tensor, weight: Tensor | None, residual: Tensor | None, eps: float, keep: bool):
+    """(output, sum, buffer): the buffer holds the 8-bit form of the normalised rows and, behind it, their 1 / rms."""
     m = _as_rows(x)
     r = None if residual is None else _as_rows(residual)
     rows, cols = m.shape
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    h = None if r is None else torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    codes = exponents = rstd = None
+    device = x.device
+    y = torch.empty(x.shape, dtype=x.dtype, device=device)
+    h = None if r is None else torch.empty(x.shape, dtype=x.dtype, device=device)
+    buffer = rstd = None
+    layout = (None, 0, None, 0)
     if keep:
-        codes, exponents = _new_codes(rows, cols, x.device)
-        rstd = torch.empty(rows, dtype=torch.float32, device=x.device)
-    with _on_device(x.device):
+        _, after = _buffer_bytes(rows, cols)
+        buffer = torch.empty(after + 4 * rows, dtype=torch.uint8, device=device)
+        layout = CompressedActivation._of((buffer,), x.shape, x.dtype)._layout()
+        rstd = buffer.data_ptr() + after
+    with _on_device(device):
         _lib.check(_lib.LIB.optimi_b200_rms_norm(
             m.data_ptr(), m.stride(0), _ptr(r), 0 if r is None else r.stride(0), _ptr(weight), rows, cols, eps,
-            _lib.DTYPE_CODE[x.dtype], y.data_ptr(), _ptr(h), _ptr(codes), codes.stride(0) if keep else 0, _ptr(exponents),
-            exponents.stride(0) if keep else 0, _ptr(rstd), _stream(x.device)))  # fmt: skip
-    return y, h, codes, exponents, rstd
+            _lib.DTYPE_CODE[x.dtype], y.data_ptr(), _ptr(h), *layout, rstd, _stream(device)))  # fmt: skip
+    return y, h, buffer
 
 
 class _RMSNorm(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, weight, residual, eps):
-        w = None if weight is None else weight.detach().contiguous()
-        y, h, codes, exponents, rstd = _norm_forward(x, w, residual, eps, True)
-        ctx.save_for_backward(codes, exponents, rstd, weight)
-        ctx.mark_non_differentiable(codes, exponents)
+    def forward(ctx, x, weight, residual, eps, kept):
+        w = None if weight is None else weight.contiguous()
+        y, h, buffer = _norm_forward(x, w, residual, eps, True)
+        kept.append(buffer)
+        ctx.save_for_backward(buffer, weight)
         ctx.set_materialize_grads(False)
-        return y, h, codes, exponents
+        return y, h
 
     @staticmethod
-    @once_differentiable
-    def backward(ctx, grad, grad_sum, *_):
-        codes, exponents, rstd, weight = ctx.saved_tensors
+    def backward(ctx, grad, grad_sum):
+        _refuse_double_backward("rms_norm")
+        buffer, weight = ctx.saved_tensors
         need_x, need_w, need_r = ctx.needs_input_grad[:3]
         if grad is None:  # only the residual was used: it passes through
             dw = torch.zeros_like(weight) if need_w else None
-            return grad_sum if need_x else None, dw, grad_sum if need_r else None, None
+            return grad_sum if need_x else None, dw, grad_sum if need_r else None, None, None
         g = _as_rows(grad)
         s = None if grad_sum is None else _as_rows(grad_sum)
-        w = None if weight is None else weight.detach().contiguous()
+        w = None if weight is None else weight.contiguous()
         rows, cols = g.shape
         dx = torch.empty(grad.shape, dtype=grad.dtype, device=grad.device) if need_x or need_r else None
-        dw = torch.empty(cols, dtype=grad.dtype, device=grad.device) if need_w else None
+        dw = torch.empty_like(w) if need_w else None
         need = _lib.LIB.optimi_b200_rms_norm_backward_workspace_bytes(rows, cols) if need_w else 0
         workspace = torch.empty(need, dtype=torch.uint8, device=grad.device) if need else None
         with _on_device(grad.device):
             _lib.check(_lib.LIB.optimi_b200_rms_norm_backward(
-                g.data_ptr(), g.stride(0), _ptr(s), 0 if s is None else s.stride(0), codes.data_ptr(), codes.stride(0),
-                exponents.data_ptr(), exponents.stride(0), rstd.data_ptr(), _ptr(w), rows, cols, _lib.DTYPE_CODE[grad.dtype],
-                _ptr(dx), _ptr(dw), _ptr(workspace), need, _stream(grad.device)))  # fmt: skip
-        return dx if need_x else None, dw, dx if need_r else None, None
+                g.data_ptr(), g.stride(0), _ptr(s), 0 if s is None else s.stride(0),
+                *CompressedActivation._of((buffer,), grad.shape, grad.dtype)._layout(), buffer.data_ptr() + _buffer_bytes(rows, cols)[1],
+                _ptr(w), rows, cols, _lib.DTYPE_CODE[grad.dtype], _ptr(dx), _ptr(dw), _ptr(workspace), need, _stream(grad.device)))  # fmt: skip
+        return dx if need_x else None, dw, dx if need_r else None, None, None
+
+
+def _refuse_double_backward(name: str) -> None:
+    # gradients are recorded inside a backward pass only under create_graph=True, and these kernels' would come out as constants
+    if torch.is_grad_enabled():
+        raise RuntimeError(f"{name}: differentiating the backward pass (create_graph=True) is not supported")
 
 
 def rms_norm(x: Tensor, weight: Tensor | None = None, residual: Tensor | None = None, *, eps: float | None = None,
@@ -310,11 +350,13 @@ def rms_norm(x: Tensor, weight: Tensor | None = None, residual: Tensor | None = 
         x.requires_grad or (weight is not None and weight.requires_grad) or (residual is not None and residual.requires_grad)
     )
     if wants_grad:
-        y, h, codes, exponents = _RMSNorm.apply(x, weight, residual, eps)
+        kept: list[Tensor] = []
+        y, h = _RMSNorm.apply(x, weight, residual, eps, kept)
+        buffer = kept[0]
     else:
         w = None if weight is None else weight.detach().contiguous()
-        y, h, codes, exponents, _ = _norm_forward(x, w, residual, eps, compress)
-    saved = None if codes is None else CompressedActivation._of(codes, exponents, x.shape, x.dtype, None if weight is None else weight.detach())
+        y, h, buffer = _norm_forward(x, w, residual, eps, compress)
+    saved = None if buffer is None else CompressedActivation._of((buffer,), x.shape, x.dtype, None if weight is None else weight.detach())
     return RMSNormOutput(y, h, saved)
 
 
@@ -323,23 +365,25 @@ class _Linear(torch.autograd.Function):
     def forward(ctx, x, weight, bias, saved):
         out = F.linear(x, weight, bias)
         ctx.shape = x.shape
-        codes = exponents = scale = None
+        ctx.keeps_weight = ctx.needs_input_grad[0]
+        keep = [weight] if ctx.keeps_weight else []
         if ctx.needs_input_grad[1]:
             if saved is None:
                 saved = compress(x)
-            codes, exponents, scale = saved.codes, saved.exponents, saved.channel_scale
-        ctx.save_for_backward(weight if ctx.needs_input_grad[0] else None, codes, exponents, scale)
+            keep += [saved.channel_scale, *saved._tensors()]
+        ctx.save_for_backward(*keep)
         return out
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, grad):
-        weight, codes, exponents, scale = ctx.saved_tensors
+        _refuse_double_backward("linear")
+        kept = list(ctx.saved_tensors)
         dx = dw = db = None
-        if ctx.needs_input_grad[0]:
-            dx = grad @ weight
+        if ctx.keeps_weight:
+            dx = grad @ kept.pop(0)
         if ctx.needs_input_grad[1]:
-            dw = weight_gradient(grad, CompressedActivation._of(codes, exponents, ctx.shape, grad.dtype, scale))
+            scale, *tensors = kept
+            dw = weight_gradient(grad, CompressedActivation._of(tensors, ctx.shape, grad.dtype, scale))
         if ctx.needs_input_grad[2]:
             db = grad.reshape(-1, grad.shape[-1]).sum(0)
         return dx, dw, db, None
