@@ -116,33 +116,82 @@ static __device__ __forceinline__ int encode(double x, int e) {
 }
 
 // ---------------------------------------------------------------------------------------------
-// chunks: C neighbouring values of a row in one thread, 16 bytes where rows begin on 16 bytes, else one value
+// chunks: 16 bytes of neighbouring values of a row in one thread
 // ---------------------------------------------------------------------------------------------
-template <typename T, int C>
+// Rows need not begin on 16 bytes (an odd width, a slice).  Fetched<T, true> and store_any move such a chunk all the same: a
+// row's chunks lie between 16-byte blocks at one distance, so a load takes the one or two blocks around it and shifts, and a
+// store gets the head of its block from the lane before.  A block is only read where a byte of it belongs to the row, and
+// no byte outside the row is written.
+template <typename T>
 struct Chunk {
-  static constexpr int kWords = C * (int)sizeof(T) >= 4 ? C * (int)sizeof(T) / 4 : 1;
+  static constexpr int C = 16 / (int)sizeof(T);
   static constexpr int kLanes = kGroup / C;  // neighbouring lanes that hold a group
-  uint32_t w[kWords];
+  uint32_t w[4];
 
   __device__ __forceinline__ void clear() {
 #pragma unroll
-    for (int i = 0; i < kWords; i++) w[i] = 0;
+    for (int i = 0; i < 4; i++) w[i] = 0;
   }
   __device__ __forceinline__ void load(const T* p) {
-    if constexpr (kWords == 4) {
-      const uint4 v = *reinterpret_cast<const uint4*>(p);
-      w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
-    } else if constexpr (sizeof(T) == 4) {
-      w[0] = __float_as_uint(*p);
+    const uint4 v = *reinterpret_cast<const uint4*>(p);
+    w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
+  }
+  __device__ __forceinline__ void store(T* p) const { *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]); }
+
+  __device__ __forceinline__ void store_value(T* p, int i) const {
+    if constexpr (sizeof(T) == 4) p[i] = __uint_as_float(w[i]);
+    else reinterpret_cast<unsigned short*>(p)[i] = (unsigned short)(w[i / 2] >> (i % 2 * 16));
+  }
+  // The first n values to p.  All lanes of a warp call it, with neighbouring chunks of one row: lane l's p is lane 0's + l * C, n is
+  // C up to some lane and 0 after the next.  n may be negative: nothing.
+  __device__ __forceinline__ void store_any(T* p, int n) const {
+    const uint32_t off = (uint32_t)reinterpret_cast<uintptr_t>(p) & 15u;  // the same in all lanes
+    n = max(0, min(n, C));
+    if (off == 0) {
+      if (n == C) {
+        store(p);
+      } else {
+#pragma unroll
+        for (int i = 0; i < C; i++)
+          if (i < n) store_value(p, i);
+      }
+      return;
+    }
+    const int lane = threadIdx.x % 32, head = (16 - (int)off) / (int)sizeof(T);  // values of a chunk that lie in its first block
+    Chunk before;
+#pragma unroll
+    for (int i = 0; i < 4; i++) before.w[i] = __shfl_up_sync(~0u, w[i], 1);
+    const int n_before = __shfl_up_sync(~0u, n, 1);
+    if (lane > 0 && n >= head) {  // then the chunk before is whole
+      uint32_t u[8] = {before.w[0], before.w[1], before.w[2], before.w[3], w[0], w[1], w[2], w[3]};
+      // the block is bytes 16 - off .. 31 - off of the two
+      const uint32_t skip = 16 - off;
+      if (skip & 8) {
+#pragma unroll
+        for (int i = 0; i < 6; i++) u[i] = u[i + 2];
+      }
+      if (skip & 4) {
+#pragma unroll
+        for (int i = 0; i < 5; i++) u[i] = u[i + 1];
+      }
+      Chunk out;
+#pragma unroll
+      for (int i = 0; i < 4; i++) out.w[i] = sizeof(T) == 2 ? __funnelshift_r(u[i], u[i + 1], (skip & 2) * 8) : u[i];
+      out.store(reinterpret_cast<T*>(reinterpret_cast<uintptr_t>(p) - off));
     } else {
-      w[0] = *reinterpret_cast<const unsigned short*>(p);
+#pragma unroll
+      for (int i = 0; i < C; i++) {
+        if (lane > 0 && i >= head && i < n_before) before.store_value(p - C, i);
+        if (i < head && i < n) store_value(p, i);
+      }
+    }
+    if (lane == 31) {
+#pragma unroll
+      for (int i = 0; i < C; i++)
+        if (i >= head && i < n) store_value(p, i);
     }
   }
-  __device__ __forceinline__ void store(T* p) const {
-    if constexpr (kWords == 4) *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
-    else if constexpr (sizeof(T) == 4) *p = __uint_as_float(w[0]);
-    else *reinterpret_cast<unsigned short*>(p) = (unsigned short)w[0];
-  }
+
   __device__ __forceinline__ float get(int i) const {
     if constexpr (sizeof(T) == 4) return __uint_as_float(w[i]);
     else if constexpr (std::is_same<T, __half>::value) return __half2float(__ushort_as_half((unsigned short)(w[i / 2] >> (i % 2 * 16))));
@@ -150,29 +199,23 @@ struct Chunk {
   }
   // v[0..C-1], rounded to T
   __device__ __forceinline__ void set(const float* v) {
-    if constexpr (sizeof(T) == 4) {
 #pragma unroll
-      for (int i = 0; i < C; i++) w[i] = __float_as_uint(v[i]);
-    } else {
-#pragma unroll
-      for (int i = 0; i < kWords; i++) {
-        const float high = C == 1 ? 0.0f : v[C == 1 ? 0 : 2 * i + 1];
-        if constexpr (std::is_same<T, __half>::value) asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(w[i]) : "f"(high), "f"(v[C == 1 ? 0 : 2 * i]));
-        else asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(w[i]) : "f"(high), "f"(v[C == 1 ? 0 : 2 * i]));
-      }
+    for (int i = 0; i < 4; i++) {
+      if constexpr (sizeof(T) == 4) w[i] = __float_as_uint(v[i]);
+      else if constexpr (std::is_same<T, __half>::value) asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(w[i]) : "f"(v[2 * i + 1]), "f"(v[2 * i]));
+      else asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(w[i]) : "f"(v[2 * i + 1]), "f"(v[2 * i]));
     }
   }
   // The largest magnitude, as fp32 bits: magnitudes compare as whole numbers, NaNs above infinity.
   __device__ __forceinline__ uint32_t amax() const {
+    uint32_t m = 0;
     if constexpr (sizeof(T) == 4) {
-      uint32_t m = 0;
 #pragma unroll
-      for (int i = 0; i < kWords; i++) m = max(m, w[i] & 0x7fffffffu);
+      for (int i = 0; i < 4; i++) m = max(m, w[i] & 0x7fffffffu);
       return m;
     } else {
-      uint32_t m = 0;
 #pragma unroll
-      for (int i = 0; i < kWords; i++) m = __vmaxu2(m, w[i] & 0x7fff7fffu);
+      for (int i = 0; i < 4; i++) m = __vmaxu2(m, w[i] & 0x7fff7fffu);
       m = max(m & 0xffffu, m >> 16);
       if constexpr (std::is_same<T, __half>::value) return __float_as_uint(__half2float(__ushort_as_half((unsigned short)m)));
       else return m << 16;
@@ -180,19 +223,70 @@ struct Chunk {
   }
 };
 
+// A chunk on its way from memory: fetch() asks for it, settle() (same arguments) is the first to need it, so that many can be under
+// way at once.  The first n values at p, zeros behind them; n may be more than a chunk or negative.
+template <typename T, bool kAny>
+struct Fetched {
+  static constexpr int C = Chunk<T>::C;
+  uint32_t u[kAny ? 8 : 4];
+
+  __device__ __forceinline__ void fetch(const T* p, int n) {
+    uint4 a = make_uint4(0, 0, 0, 0), b = make_uint4(0, 0, 0, 0);
+    if constexpr (!kAny) {
+      if (n > 0) a = *reinterpret_cast<const uint4*>(p);
+    } else {
+      const uint32_t off = (uint32_t)reinterpret_cast<uintptr_t>(p) & 15u;
+      const uint4* block = reinterpret_cast<const uint4*>(reinterpret_cast<uintptr_t>(p) - off);
+      if (n > 0) a = block[0];
+      if (n > 0 && off + (uint32_t)min(n, C) * (uint32_t)sizeof(T) > 16) b = block[1];
+      u[4] = b.x, u[5] = b.y, u[6] = b.z, u[7] = b.w;
+    }
+    u[0] = a.x, u[1] = a.y, u[2] = a.z, u[3] = a.w;
+  }
+  __device__ __forceinline__ Chunk<T> settle(const T* p, int n) const {
+    Chunk<T> v;
+    if constexpr (!kAny) {
+#pragma unroll
+      for (int i = 0; i < 4; i++) v.w[i] = u[i];
+    } else {
+      const uint32_t off = (uint32_t)reinterpret_cast<uintptr_t>(p) & 15u;
+      uint32_t s[8];
+#pragma unroll
+      for (int i = 0; i < 8; i++) s[i] = u[i];
+      if (off & 8) {
+#pragma unroll
+        for (int i = 0; i < 6; i++) s[i] = s[i + 2];
+      }
+      if (off & 4) {
+#pragma unroll
+        for (int i = 0; i < 5; i++) s[i] = s[i + 1];
+      }
+#pragma unroll
+      for (int i = 0; i < 4; i++) v.w[i] = sizeof(T) == 2 ? __funnelshift_r(s[i], s[i + 1], (off & 2) * 8) : s[i];
+      if (n < C) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+          if constexpr (sizeof(T) == 4) v.w[i] = i < n ? v.w[i] : 0;
+          else v.w[i] = 2 * i + 1 < n ? v.w[i] : 2 * i < n ? v.w[i] & 0xffffu : 0;
+        }
+      }
+    }
+    return v;
+  }
+};
+
 // The largest of a group's magnitudes, in all its lanes.
 template <int kLanes>
 static __device__ __forceinline__ uint32_t group_max(uint32_t m) {
-  if constexpr (kLanes == 32) return __reduce_max_sync(~0u, m);
 #pragma unroll
   for (int d = 1; d < kLanes; d *= 2) m = max(m, __shfl_xor_sync(~0u, m, d));
   return m;
 }
 
-// C codes, in bytes.
+// C (8 or 4) codes.
 template <int C>
 struct CodeChunk {
-  static constexpr int kWords = C >= 4 ? C / 4 : 1;
+  static constexpr int kWords = C / 4;
   uint32_t w[kWords];
 
   // From values in fp32 that are at most 127.5 in a unit of 2^(e - 127), or more where e was held at its largest.  One fused
@@ -218,13 +312,9 @@ struct CodeChunk {
     set(c);
   }
   __device__ __forceinline__ void set(const uint32_t* c) {
-    if constexpr (C == 1) {
-      w[0] = c[0];
-    } else {
 #pragma unroll
-      for (int i = 0; i < kWords; i++)
-        w[i] = __byte_perm(__byte_perm(c[4 * i], c[4 * i + 1], 0x0040), __byte_perm(c[4 * i + 2], c[4 * i + 3], 0x0040), 0x5410);
-    }
+    for (int i = 0; i < kWords; i++)
+      w[i] = __byte_perm(__byte_perm(c[4 * i], c[4 * i + 1], 0x0040), __byte_perm(c[4 * i + 2], c[4 * i + 3], 0x0040), 0x5410);
   }
   __device__ __forceinline__ void clear() {
 #pragma unroll
@@ -234,16 +324,13 @@ struct CodeChunk {
     if constexpr (C == 8) {
       const uint2 v = *reinterpret_cast<const uint2*>(p);
       w[0] = v.x, w[1] = v.y;
-    } else if constexpr (C == 4) {
-      w[0] = *reinterpret_cast<const uint32_t*>(p);
     } else {
-      w[0] = *reinterpret_cast<const uint8_t*>(p);
+      w[0] = *reinterpret_cast<const uint32_t*>(p);
     }
   }
   __device__ __forceinline__ void store(int8_t* p) const {
     if constexpr (C == 8) *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
-    else if constexpr (C == 4) *reinterpret_cast<uint32_t*>(p) = w[0];
-    else *p = (int8_t)w[0];
+    else *reinterpret_cast<uint32_t*>(p) = w[0];
   }
   // Code i as fp32: the byte with its sign bit flipped, set into the low bits of 2^23, is 2^23 + 128 + code.
   __device__ __forceinline__ float get(int i) const {

@@ -11,80 +11,81 @@ namespace act {
 // together), kUnroll items a thread are loaded before the first is used, and nothing is read or written twice.
 constexpr int kBlock = 256, kUnroll = 4;
 
-// Where chunk `item` lies: rows of `chunks` chunks, the last group of a row filled up.  With kFlat rows follow one another without
-// a gap and are whole groups, so that a tensor is one long row and nothing is divided.
-template <int C, bool kFlat>
-struct Place {
-  int64_t row, col;
-  __device__ __forceinline__ Place(int64_t item, int64_t chunks) {
-    if constexpr (kFlat) {
-      row = 0, col = item * C;
-    } else if (item < (1ll << 31) && chunks < (1ll << 31)) {
-      row = (uint32_t)item / (uint32_t)chunks, col = ((uint32_t)item - (uint32_t)row * (uint32_t)chunks) * (int64_t)C;
-    } else {
-      row = item / chunks, col = (item - row * chunks) * C;
-    }
+static __device__ __forceinline__ void divide(int64_t a, int64_t b, int64_t* quotient, int64_t* rest) {
+  if (((a | b) >> 31) == 0) {
+    *quotient = (uint32_t)a / (uint32_t)b;
+    *rest = (uint32_t)a % (uint32_t)b;
+  } else {
+    *quotient = a / b;
+    *rest = a % b;
   }
-};
+}
 
-template <typename T, int C, bool kFlat>
+// How the rows of the 16-bit or 32-bit tensor lie.  kFlat: whole groups, one row after another without a gap, so that it is one
+// long row and nothing is divided.  kRows: every row begins on 16 bytes and is whole chunks.  kAny: neither.
+enum Lie : int { kFlat, kRows, kAny };
+
+template <typename T, int kLie>
 __global__ void __launch_bounds__(kBlock) compress_kernel(const T* __restrict__ x, int64_t items, int64_t chunks, int64_t cols, int64_t stride,
                                                           int8_t* __restrict__ codes, int64_t pitch, uint8_t* __restrict__ exponents,
                                                           int64_t epitch) {
-  constexpr int kLanes = Chunk<T, C>::kLanes;
+  constexpr int C = Chunk<T>::C, kLanes = Chunk<T>::kLanes;
   const int64_t first = (int64_t)blockIdx.x * (kBlock * kUnroll) + threadIdx.x;
-  Chunk<T, C> v[kUnroll];
+  Fetched<T, kLie == kAny> in[kUnroll];
+  int64_t row[kUnroll], col[kUnroll];
+  int n[kUnroll];
 #pragma unroll
   for (int u = 0; u < kUnroll; u++) {
     const int64_t item = first + u * kBlock;
-    v[u].clear();
-    if (item < items) {
-      const Place<C, kFlat> at(item, chunks);
-      if (kFlat || at.col < cols) v[u].load(x + at.row * stride + at.col);
-    }
+    row[u] = 0, col[u] = item;
+    if (kLie != kFlat) divide(item, chunks, &row[u], &col[u]);
+    col[u] *= C;
+    n[u] = item >= items ? 0 : kLie == kFlat ? C : (int)min((int64_t)C, cols - col[u]);
+    in[u].fetch(x + row[u] * stride + col[u], n[u]);
   }
 #pragma unroll
   for (int u = 0; u < kUnroll; u++) {
-    const int64_t item = first + u * kBlock;
-    const int e = group_exponent<T>(group_max<kLanes>(v[u].amax()));
+    const Chunk<T> v = in[u].settle(x + row[u] * stride + col[u], n[u]);
+    const int e = group_exponent<T>(group_max<kLanes>(v.amax()));
     float f[C];
 #pragma unroll
-    for (int i = 0; i < C; i++) f[i] = v[u].get(i);
+    for (int i = 0; i < C; i++) f[i] = v.get(i);
     CodeChunk<C> c;
     c.template encode<T>(f, e);
-    if (item < items) {
-      const Place<C, kFlat> at(item, chunks);
-      c.store(codes + at.row * pitch + at.col);
-      if (threadIdx.x % kLanes == 0) exponents[at.row * epitch + at.col / kGroup] = (uint8_t)e;
+    if (first + u * kBlock < items) {
+      c.store(codes + row[u] * pitch + col[u]);
+      if (threadIdx.x % kLanes == 0) exponents[row[u] * epitch + col[u] / kGroup] = (uint8_t)e;
     }
   }
 }
 
-template <typename T, int C, bool kFlat, bool kScaled>
+template <typename T, int kLie, bool kScaled>
 __global__ void __launch_bounds__(kBlock) decompress_kernel(const int8_t* __restrict__ codes, int64_t pitch, const uint8_t* __restrict__ exponents,
                                                             int64_t epitch, const T* __restrict__ channel_scale, int64_t items,
                                                             int64_t chunks, int64_t cols, T* __restrict__ out) {
+  constexpr int C = Chunk<T>::C;
   const int64_t first = (int64_t)blockIdx.x * (kBlock * kUnroll) + threadIdx.x;
   CodeChunk<C> c[kUnroll];
   uint32_t e[kUnroll];
+  int64_t row[kUnroll], col[kUnroll];
 #pragma unroll
   for (int u = 0; u < kUnroll; u++) {
     const int64_t item = first + u * kBlock;
+    row[u] = 0, col[u] = item;
+    if (kLie != kFlat) divide(item, chunks, &row[u], &col[u]);
+    col[u] *= C;
     c[u].clear(), e[u] = 0;
     if (item < items) {
-      const Place<C, kFlat> at(item, chunks);
-      c[u].load(codes + at.row * pitch + at.col);
-      e[u] = exponents[at.row * epitch + at.col / kGroup];
+      c[u].load(codes + row[u] * pitch + col[u]);
+      e[u] = exponents[row[u] * epitch + col[u] / kGroup];
     }
   }
 #pragma unroll
   for (int u = 0; u < kUnroll; u++) {
-    const int64_t item = first + u * kBlock;
-    if (item >= items) return;
-    const Place<C, kFlat> at(item, chunks);
-    if (!kFlat && at.col >= cols) continue;
-    Chunk<T, C> v;
-    if constexpr (sizeof(T) == 2 && C == 8 && !kScaled) {
+    if (first + u * kBlock >= items) return;
+    if (kLie != kFlat && col[u] >= cols) continue;
+    Chunk<T> v;
+    if constexpr (sizeof(T) == 2 && !kScaled) {
       const uint32_t s = scale_pair<T>(e[u], 0x4040);
 #pragma unroll
       for (int i = 0; i < 4; i++) v.w[i] = code_pair<T>(c[u].w[i / 2], i % 2 ? 0x4342 : 0x4140, s);
@@ -94,11 +95,65 @@ __global__ void __launch_bounds__(kBlock) decompress_kernel(const int8_t* __rest
 #pragma unroll
       for (int i = 0; i < C; i++) {
         f[i] = __fmul_rn(c[u].get(i), s);
-        if (kScaled) f[i] = __fmul_rn(f[i], to_f32(channel_scale[(kFlat ? at.col % cols : at.col) + i]));
+        if (kScaled) f[i] = __fmul_rn(f[i], to_f32(channel_scale[(kLie == kFlat ? col[u] % cols : col[u]) + i]));
       }
       v.set(f);
     }
-    v.store(out + at.row * cols + at.col);
+    v.store(out + row[u] * cols + col[u]);
+  }
+}
+
+// The same for rows that begin anywhere.  The result has no gaps, so an item is one 16-byte block of it as a whole; its codes lie at
+// any byte of a row (whose pitch is a multiple of 32), and a block that reaches into the next row takes them one by one.
+template <typename T, bool kScaled>
+__global__ void __launch_bounds__(kBlock) decompress_any_kernel(const int8_t* __restrict__ codes, int64_t pitch, const uint8_t* __restrict__ exponents,
+                                                                int64_t epitch, const T* __restrict__ channel_scale, int64_t values,
+                                                                int64_t cols, T* __restrict__ out) {
+  constexpr int C = Chunk<T>::C;
+  const int64_t first = (int64_t)blockIdx.x * (kBlock * kUnroll) + threadIdx.x;
+#pragma unroll
+  for (int u = 0; u < kUnroll; u++) {
+    const int64_t at = (first + u * kBlock) * C;
+    if (at >= values) return;
+    int64_t row, col;
+    divide(at, cols, &row, &col);
+    float f[C];
+    if (col + C <= cols) {
+      const uint32_t* words = reinterpret_cast<const uint32_t*>(codes + row * pitch + (col & ~3ll));
+      const uint32_t shift = (uint32_t)(col & 3) * 8;
+      uint32_t w[C / 4 + 1];
+#pragma unroll
+      for (int i = 0; i < C / 4; i++) w[i] = words[i];
+      w[C / 4] = shift ? words[C / 4] : 0;  // the last code asked for lies there
+      CodeChunk<C> c;
+#pragma unroll
+      for (int i = 0; i < C / 4; i++) c.w[i] = __funnelshift_r(w[i], w[i + 1], shift);
+      const uint8_t* group = exponents + row * epitch + col / kGroup;
+      const int in = (int)(col % kGroup);
+      const float low = power_of(group[0]), high = power_of(group[(in + C - 1) / kGroup]);
+#pragma unroll
+      for (int i = 0; i < C; i++) f[i] = __fmul_rn(c.get(i), in + i < kGroup ? low : high);
+    } else {
+#pragma unroll
+      for (int i = 0; i < C; i++) {
+        int64_t r, k;
+        divide(min(at + i, values - 1), cols, &r, &k);
+        f[i] = __fmul_rn((float)codes[r * pitch + k], power_of(exponents[r * epitch + k / kGroup]));
+      }
+    }
+    if constexpr (kScaled) {
+#pragma unroll
+      for (int i = 0; i < C; i++) f[i] = __fmul_rn(f[i], to_f32(channel_scale[(col + i) % cols]));
+    }
+    Chunk<T> v;
+    v.set(f);
+    if (at + C <= values) {
+      v.store(out + at);
+    } else {
+#pragma unroll
+      for (int i = 0; i < C; i++)
+        if (at + i < values) v.store_value(out + at, i);
+    }
   }
 }
 
@@ -134,49 +189,75 @@ static __device__ __forceinline__ F row_sum(F v, F (*part)[P / 32], int turn, in
   return v;
 }
 
-template <typename T, int C, int P, int K, bool kKeep>
-__global__ void __launch_bounds__(P < 128 ? 128 : P)
+template <typename T, bool kAny>
+static __device__ __forceinline__ void store_chunk(const Chunk<T>& v, T* row, int c, int cols) {
+  if constexpr (kAny) v.store_any(row + c, cols - c);
+  else if (c < cols) v.store(row + c);
+}
+
+template <typename T, int P, int K, bool kAny, bool kKeep>
+__global__ void __launch_bounds__(P < 128 ? 128 : P, kAny && K <= 2 ? 1024 / (P < 128 ? 128 : P) : 0)
     rms_norm_kernel(const T* __restrict__ x, int64_t xs, const T* __restrict__ residual, int64_t rs, const T* __restrict__ weight,
                     int64_t rows, int cols, double eps, T* __restrict__ y, T* __restrict__ sum, int8_t* __restrict__ codes, int64_t pitch,
                     uint8_t* __restrict__ exponents, int64_t epitch, float* __restrict__ rstd_out) {
   using F = typename Wide<T>::type;
-  using Values = Chunk<T, C>;
-  constexpr int kGroups = (P < 128 ? 128 : P) / P;
+  using Values = Chunk<T>;
+  constexpr int C = Values::C, kGroups = (P < 128 ? 128 : P) / P;
   __shared__ F part[kGroups][2][P / 32];
   const int group = threadIdx.x / P, t = threadIdx.x % P;
   const int padded = (cols + kGroup - 1) / kGroup * kGroup;
   Values w[K];
+  if (weight) {
 #pragma unroll
-  for (int k = 0; k < K; k++) {
-    const int c = (k * P + t) * C;
-    if (weight && c < cols) w[k].load(weight + c);
+    for (int k = 0; k < K; k++) {
+      const int c = (k * P + t) * C;
+      Fetched<T, kAny> in;
+      in.fetch(weight + c, cols - c);
+      w[k] = in.settle(weight + c, cols - c);
+    }
   }
   int turn = 0;
   for (int64_t row = (int64_t)blockIdx.x * kGroups + group; row < rows; row += (int64_t)gridDim.x * kGroups, turn++) {
     Values h[K];
     F ss = 0;
+    const auto add = [&](int k, const Values& r) {
+      float f[C];
 #pragma unroll
-    for (int k = 0; k < K; k++) {
-      const int c = (k * P + t) * C;
-      h[k].clear();
-      if (c < cols) h[k].load(x + row * xs + c);
-    }
-    if (residual) {
-      Values r[K];
+      for (int i = 0; i < C; i++) f[i] = __fadd_rn(h[k].get(i), r.get(i));
+      h[k].set(f);
+      store_chunk<T, kAny>(h[k], sum + row * cols, (k * P + t) * C, cols);
+    };
+    if constexpr (kAny) {
+      Fetched<T, true> in[K], more[K];
 #pragma unroll
       for (int k = 0; k < K; k++) {
         const int c = (k * P + t) * C;
-        r[k].clear();
-        if (c < cols) r[k].load(residual + row * rs + c);
+        in[k].fetch(x + row * xs + c, cols - c);
+        more[k].fetch(residual + row * rs + c, residual ? cols - c : 0);
       }
 #pragma unroll
       for (int k = 0; k < K; k++) {
         const int c = (k * P + t) * C;
-        float f[C];
+        h[k] = in[k].settle(x + row * xs + c, cols - c);
+        if (residual) add(k, more[k].settle(residual + row * rs + c, cols - c));
+      }
+    } else {
 #pragma unroll
-        for (int i = 0; i < C; i++) f[i] = __fadd_rn(h[k].get(i), r[k].get(i));
-        h[k].set(f);
-        if (c < cols) h[k].store(sum + row * cols + c);
+      for (int k = 0; k < K; k++) {
+        const int c = (k * P + t) * C;
+        h[k].clear();
+        if (c < cols) h[k].load(x + row * xs + c);
+      }
+      if (residual) {
+        Values r[K];
+#pragma unroll
+        for (int k = 0; k < K; k++) {
+          const int c = (k * P + t) * C;
+          r[k].clear();
+          if (c < cols) r[k].load(residual + row * rs + c);
+        }
+#pragma unroll
+        for (int k = 0; k < K; k++) add(k, r[k]);
       }
     }
 #pragma unroll
@@ -202,11 +283,11 @@ __global__ void __launch_bounds__(P < 128 ? 128 : P)
       }
       Values out;
       out.set(f);
-      if (c < cols) out.store(y + row * cols + c);
+      store_chunk<T, kAny>(out, y + row * cols, c, cols);
       if constexpr (kKeep) {
         // rounding keeps the order of magnitudes, so the largest |h| times rstd is the largest |xn|
-        const F top = (F)__uint_as_float(h[k].amax()) * rstd;
-        const int e = exponent_of<T, F>(group_max<Values::kLanes>(magnitude(top)));
+        const F top = (F)__uint_as_float(group_max<Values::kLanes>(h[k].amax())) * rstd;
+        const int e = exponent_of<T, F>(magnitude(top));
         CodeChunk<C> code;
         code.template encode<T>(n, e);
         if (c < padded) {
@@ -272,77 +353,115 @@ __global__ void long_rms_norm_kernel(const T* __restrict__ x, int64_t xs, const 
 //
 // A block keeps its threads' columns of dw in registers over all its rows, and leaves one line of partial sums in the workspace
 // (its row groups added up in order in shared memory); a second kernel adds up the lines in order.  Few blocks, so few lines.
-template <typename T, int C, int P, int K, int kThreads>
-__global__ void __launch_bounds__(kThreads)
+// The next row is asked for before this one is reduced (kAhead), so that loads are always under way.  Long rows (K > 2) have no
+// registers for that, nor for the weight, which they read again for every row, nor for dsum, asked for after the first pass.
+template <typename T, int K, bool kAny>
+struct BackwardRow {
+  Fetched<T, kAny> g[K], s[K];
+  CodeChunk<Chunk<T>::C> code[K];
+  uint32_t e[K];
+  float r;
+};
+
+template <typename T, int P, int K, bool kAny>
+__global__ void __launch_bounds__(512, 1)
     rms_norm_backward_kernel(const T* __restrict__ grad, int64_t gs, const T* __restrict__ grad_sum, int64_t hs, const int8_t* __restrict__ codes,
                              int64_t pitch, const uint8_t* __restrict__ exponents, int64_t epitch, const float* __restrict__ rstd,
                              const T* __restrict__ weight, int64_t rows, int cols, T* __restrict__ dx, float* __restrict__ lines) {
-  using Values = Chunk<T, C>;
-  constexpr int kGroups = kThreads / P;
+  using Values = Chunk<T>;
+  constexpr bool kAhead = K <= 2;
+  constexpr int C = Values::C, kThreads = 512, kGroups = kThreads / P;
   __shared__ float part[kGroups][2][P / 32];
-  extern __shared__ float line[];
+  __shared__ float sums[kGroups > 1 ? kGroups : 1][kGroups > 1 ? P * K * C + 4 : 1];
   const int group = threadIdx.x / P, t = threadIdx.x % P;
   Values w[K];
   float dw[K][C];
+  const auto weights = [&](int k) {
+    const int c = (k * P + t) * C;
+    Fetched<T, kAny> in;
+    in.fetch(weight + c, weight ? cols - c : 0);
+    return in.settle(weight + c, weight ? cols - c : 0);
+  };
 #pragma unroll
   for (int k = 0; k < K; k++) {
-    const int c = (k * P + t) * C;
-    w[k].clear();
-    if (weight && c < cols) w[k].load(weight + c);
+    if constexpr (kAhead) w[k] = weights(k);
 #pragma unroll
     for (int i = 0; i < C; i++) dw[k][i] = 0.0f;
   }
-  int turn = 0;
-  for (int64_t row = (int64_t)blockIdx.x * kGroups + group; row < rows; row += (int64_t)gridDim.x * kGroups, turn++) {
-    Values g[K], s[K];
-    CodeChunk<C> code[K];
-    uint32_t e[K];
-    const float r = rstd[row];
+  const int64_t step = (int64_t)gridDim.x * kGroups;
+  const auto ask_sum = [&](int64_t row, BackwardRow<T, K, kAny>& v) {
 #pragma unroll
     for (int k = 0; k < K; k++) {
       const int c = (k * P + t) * C;
-      g[k].clear(), code[k].clear(), e[k] = 0;
-      if (c < cols) {
-        g[k].load(grad + row * gs + c);
-        code[k].load(codes + row * pitch + c);
-        e[k] = exponents[row * epitch + c / kGroup];
-      }
+      v.s[k].fetch(grad_sum + row * hs + c, grad_sum && dx ? cols - c : 0);
     }
-    if (grad_sum && dx) {
+  };
+  const auto ask = [&](int64_t row, BackwardRow<T, K, kAny>& v) {
+    if (row >= rows) return;
+    v.r = rstd[row];
 #pragma unroll
-      for (int k = 0; k < K; k++) {
-        const int c = (k * P + t) * C;
-        if (c < cols) s[k].load(grad_sum + row * hs + c);
+    for (int k = 0; k < K; k++) {
+      const int c = (k * P + t) * C;
+      v.g[k].fetch(grad + row * gs + c, cols - c);
+      v.code[k].clear(), v.e[k] = 0;
+      if (c < cols) {
+        v.code[k].load(codes + row * pitch + c);
+        v.e[k] = exponents[row * epitch + c / kGroup];
       }
     }
+    if constexpr (kAhead) ask_sum(row, v);
+  };
+  int turn = 0;
+  BackwardRow<T, K, kAny> v, next;
+  int64_t row = (int64_t)blockIdx.x * kGroups + group;
+  ask(row, v);
+  for (; row < rows; row += step, turn++) {
+    if constexpr (kAhead) ask(row + step, next);
+    Values g[K];
     float m = 0;
 #pragma unroll
     for (int k = 0; k < K; k++) {
-      const float unit = power_of((int)e[k]);
-#pragma unroll
-      for (int i = 0; i < C; i++) {
-        const float n = __fmul_rn(code[k].get(i), unit), v = g[k].get(i);
-        dw[k][i] = __fmaf_rn(v, n, dw[k][i]);
-        m = __fmaf_rn(weight ? __fmul_rn(v, w[k].get(i)) : v, n, m);
-      }
-    }
-    if (!dx) continue;
-    m = row_sum<P, float>(m, part[group], turn, group) / (float)cols;
-#pragma unroll
-    for (int k = 0; k < K; k++) {
       const int c = (k * P + t) * C;
-      const float unit = power_of((int)e[k]);
-      float f[C];
+      g[k] = v.g[k].settle(grad + row * gs + c, cols - c);
+      const float unit = power_of((int)v.e[k]);
+      Values wk;
+      if constexpr (kAhead) wk = w[k];
+      else wk = weights(k);
 #pragma unroll
       for (int i = 0; i < C; i++) {
-        const float n = __fmul_rn(code[k].get(i), unit), v = g[k].get(i);
-        f[i] = __fmul_rn(r, __fmaf_rn(-n, m, weight ? __fmul_rn(v, w[k].get(i)) : v));
-        if (grad_sum) f[i] = __fadd_rn(f[i], s[k].get(i));
+        const float n = __fmul_rn(v.code[k].get(i), unit), d = g[k].get(i);
+        dw[k][i] = __fmaf_rn(d, n, dw[k][i]);
+        m = __fmaf_rn(weight ? __fmul_rn(d, wk.get(i)) : d, n, m);
       }
-      Values out;
-      out.set(f);
-      if (c < cols) out.store(dx + row * cols + c);
     }
+    if (dx) {
+      if constexpr (!kAhead) ask_sum(row, v);
+      m = row_sum<P, float>(m, part[group], turn, group) / (float)cols;
+#pragma unroll
+      for (int k = 0; k < K; k++) {
+        const int c = (k * P + t) * C;
+        const float unit = power_of((int)v.e[k]);
+        Values wk;
+        if constexpr (kAhead) wk = w[k];
+        else wk = weights(k);
+        float f[C];
+#pragma unroll
+        for (int i = 0; i < C; i++) {
+          const float n = __fmul_rn(v.code[k].get(i), unit), d = g[k].get(i);
+          f[i] = __fmul_rn(v.r, __fmaf_rn(-n, m, weight ? __fmul_rn(d, wk.get(i)) : d));
+        }
+        if (grad_sum) {
+          const Values s = v.s[k].settle(grad_sum + row * hs + c, cols - c);
+#pragma unroll
+          for (int i = 0; i < C; i++) f[i] = __fadd_rn(f[i], s.get(i));
+        }
+        Values out;
+        out.set(f);
+        store_chunk<T, kAny>(out, dx + row * cols, c, cols);
+      }
+    }
+    if constexpr (kAhead) v = next;
+    else ask(row + step, v);
   }
   if (!lines) return;
   if constexpr (kGroups == 1) {
@@ -353,21 +472,19 @@ __global__ void __launch_bounds__(kThreads)
         const int c = (k * P + t) * C + i;
         if (c < cols) lines[(int64_t)blockIdx.x * cols + c] = dw[k][i];
       }
-    return;
-  }
-  for (int j = 0; j < kGroups; j++) {
-    if (j == group) {
+  } else {
 #pragma unroll
-      for (int k = 0; k < K; k++)
+    for (int k = 0; k < K; k++)
 #pragma unroll
-        for (int i = 0; i < C; i++) {
-          const int c = (k * P + t) * C + i;
-          if (c < cols) line[c] = j ? line[c] + dw[k][i] : dw[k][i];
-        }
-    }
+      for (int i = 0; i < C; i++) sums[group][(k * P + t) * C + i] = dw[k][i];
     __syncthreads();
+    for (int c = threadIdx.x; c < cols; c += kThreads) {
+      float s = sums[0][c];
+#pragma unroll
+      for (int j = 1; j < kGroups; j++) s += sums[j][c];
+      lines[(int64_t)blockIdx.x * cols + c] = s;
+    }
   }
-  for (int c = threadIdx.x; c < cols; c += kThreads) lines[(int64_t)blockIdx.x * cols + c] = line[c];
 }
 
 template <typename T>
@@ -422,42 +539,39 @@ constexpr int kLongBlocks = 148 * 4;
 // Whether rows from `p` on, `stride` apart, begin on 16 bytes.
 static bool rows_aligned(const void* p, int64_t stride, int64_t rows, int size) { return aligned(p, 16) && (rows <= 1 || stride * size % 16 == 0); }
 
-// How a row is dealt out: P threads with K chunks of C values each.  K = 0: too long for registers.
+// How a row is dealt out: P threads with K chunks each, K at most `most` as long as 512 threads are enough.  K = 0: too long for
+// registers.  16384 x 4096 bf16, K = 1, 2, 4: forward 141, 108, 100 us; backward 113, 90, 136 us (for 4 there are no registers to
+// ask ahead); forward with rows that begin anywhere, 4096 x 4095: 59, 51, 61 us.
+constexpr int kForwardChunks = 4, kForwardAnyChunks = 2, kBackwardChunks = 2;
+
 struct Deal {
-  int C, P, K;
+  int P, K;
 };
 
-static Deal deal_of(int64_t cols, int size, bool vectors) {
+static Deal deal_of(int64_t cols, int size, int most) {
+  const int64_t chunks = round_up(cols, kGroup) * size / 16;
   Deal d;
-  d.C = vectors && cols % (16 / size) == 0 ? 16 / size : 1;
-  const int64_t chunks = round_up(cols, kGroup) / d.C;
-  const int most = d.C == 1 ? 16 : 4;
-  d.P = chunks <= 32 * most ? 32 : chunks <= 128 * most ? 128 : chunks <= 256 * most ? 256 : chunks <= 512 * most ? 512 : 1024;
+  d.P = chunks <= 32 * most ? 32 : chunks <= 64 * most ? 64 : chunks <= 128 * most ? 128 : chunks <= 256 * most ? 256 : 512;
   const int64_t k = (chunks + d.P - 1) / d.P;
-  d.K = k > most ? 0 : d.C == 1 ? (k <= 4 ? 4 : 16) : k <= 1 ? 1 : k <= 2 ? 2 : 4;
+  d.K = k <= 2 ? (int)k : k <= 4 ? 4 : k <= 8 && size == 4 ? 8 : 0;
   return d;
 }
 
-// Calls f with C, P and K as constants, for every deal that deal_of makes.
-template <typename T, typename F>
+// Calls f with P and K as constants, for every deal that deal_of makes.
+template <typename T, int most, typename F>
 static void with_deal(const Deal& d, F f) {
-  constexpr int V = 16 / (int)sizeof(T);
-#define CASE(c, p, k) \
-  if (d.C == c && d.P == p && d.K == k) return f(std::integral_constant<int, c>(), std::integral_constant<int, p>(), std::integral_constant<int, k>())
-  CASE(V, 32, 1);
-  CASE(V, 32, 2);
-  CASE(V, 32, 4);
-  CASE(V, 128, 2);
-  CASE(V, 128, 4);
-  CASE(V, 256, 4);
-  CASE(V, 512, 4);
-  CASE(V, 1024, 4);
-  CASE(1, 32, 4);
-  CASE(1, 32, 16);
-  CASE(1, 128, 16);
-  CASE(1, 256, 16);
-  CASE(1, 512, 16);
-  CASE(1, 1024, 16);
+#define CASE(p, k) \
+  if (d.P == p && d.K == k) return f(std::integral_constant<int, p>(), std::integral_constant<int, k>())
+  CASE(32, 1);
+  if constexpr (most >= 2) CASE(32, 2);
+  if constexpr (most == 4) CASE(32, 4);
+  CASE(64, most);
+  CASE(128, most);
+  CASE(256, most);
+  if constexpr (most < 2) CASE(512, 1);
+  if constexpr (most <= 2) CASE(512, 2);
+  CASE(512, 4);
+  if constexpr (sizeof(T) == 4) CASE(512, 8);
 #undef CASE
 }
 
@@ -481,34 +595,38 @@ static int check_shape(const char* fn, int64_t rows, int64_t cols, int dtype) {
   return OPTIMI_OK;
 }
 
-template <typename T, int C>
+template <typename T>
 static void launch_compress(const void* x, int64_t stride, int64_t rows, int64_t cols, void* codes, int64_t pitch, void* exponents,
                             int64_t epitch, cudaStream_t s) {
+  constexpr int C = Chunk<T>::C;
   const int64_t chunks = round_up(cols, kGroup) / C, items = rows * chunks;
-  const bool flat = rows == 1 ? cols % kGroup == 0 : cols % kGroup == 0 && stride == cols && pitch == cols && epitch * kGroup == cols;
+  const bool regular = cols % C == 0 && rows_aligned(x, stride, rows, sizeof(T));
+  const bool flat = regular && cols % kGroup == 0 && (rows == 1 || (stride == cols && pitch == cols && epitch * kGroup == cols));
   const unsigned blocks = (unsigned)((items + kBlock * kUnroll - 1) / (kBlock * kUnroll));
-  if (flat)
-    compress_kernel<T, C, true><<<blocks, kBlock, 0, s>>>((const T*)x, items, chunks, cols, stride, (int8_t*)codes, pitch, (uint8_t*)exponents, epitch);
-  else
-    compress_kernel<T, C, false><<<blocks, kBlock, 0, s>>>((const T*)x, items, chunks, cols, stride, (int8_t*)codes, pitch, (uint8_t*)exponents, epitch);
+#define LAUNCH(lie)                                                                                                             \
+  compress_kernel<T, lie><<<blocks, kBlock, 0, s>>>((const T*)x, items, chunks, cols, stride, (int8_t*)codes, pitch, (uint8_t*)exponents, epitch)
+  if (flat) LAUNCH(kFlat);
+  else if (regular) LAUNCH(kRows);
+  else LAUNCH(kAny);
+#undef LAUNCH
 }
 
-template <typename T, int C>
+template <typename T, bool kScaled>
 static void launch_decompress(const void* codes, int64_t pitch, const void* exponents, int64_t epitch, const void* scale, int64_t rows,
                               int64_t cols, void* out, cudaStream_t s) {
-  const int64_t chunks = round_up(cols, kGroup) / C, items = rows * chunks;
-  const bool flat = rows == 1 ? cols % kGroup == 0 : cols % kGroup == 0 && pitch == cols && epitch * kGroup == cols;
+  constexpr int C = Chunk<T>::C;
+  const bool regular = cols % C == 0;
+  const bool flat = regular && cols % kGroup == 0 && (rows == 1 || (pitch == cols && epitch * kGroup == cols));
+  const int64_t chunks = round_up(cols, kGroup) / C, items = regular ? rows * chunks : (rows * cols + C - 1) / C;
   const unsigned blocks = (unsigned)((items + kBlock * kUnroll - 1) / (kBlock * kUnroll));
-#define LAUNCH(is_flat, is_scaled)                                                                                                       \
-  decompress_kernel<T, C, is_flat, is_scaled><<<blocks, kBlock, 0, s>>>((const int8_t*)codes, pitch, (const uint8_t*)exponents, epitch, \
-                                                                        (const T*)scale, items, chunks, cols, (T*)out)
-  if (flat) {
-    if (scale) LAUNCH(true, true);
-    else LAUNCH(true, false);
-  } else {
-    if (scale) LAUNCH(false, true);
-    else LAUNCH(false, false);
-  }
+#define LAUNCH(lie)                                                                                                             \
+  decompress_kernel<T, lie, kScaled><<<blocks, kBlock, 0, s>>>((const int8_t*)codes, pitch, (const uint8_t*)exponents, epitch,      \
+                                                               (const T*)scale, items, chunks, cols, (T*)out)
+  if (flat) LAUNCH(kFlat);
+  else if (regular) LAUNCH(kRows);
+  else
+    decompress_any_kernel<T, kScaled><<<blocks, kBlock, 0, s>>>((const int8_t*)codes, pitch, (const uint8_t*)exponents, epitch, (const T*)scale,
+                                                                rows * cols, cols, (T*)out);
 #undef LAUNCH
 }
 
@@ -530,13 +648,7 @@ int optimi_b200_compress(const void* x, int64_t x_stride, int64_t rows, int64_t 
   rc = check_codes(fn, codes, code_pitch, exponents, exponent_pitch, cols);
   if (rc == OPTIMI_OK) rc = check_items(fn, rows, cols);
   if (rc != OPTIMI_OK) return rc;
-  FOR_DTYPE(dtype, {
-    constexpr int V = 16 / (int)sizeof(T);
-    if (cols % V == 0 && rows_aligned(x, x_stride, rows, sizeof(T)))
-      launch_compress<T, V>(x, x_stride, rows, cols, codes, code_pitch, exponents, exponent_pitch, (cudaStream_t)stream);
-    else
-      launch_compress<T, 1>(x, x_stride, rows, cols, codes, code_pitch, exponents, exponent_pitch, (cudaStream_t)stream);
-  });
+  FOR_DTYPE(dtype, launch_compress<T>(x, x_stride, rows, cols, codes, code_pitch, exponents, exponent_pitch, (cudaStream_t)stream));
   return launched(fn);
 }
 
@@ -545,17 +657,15 @@ int optimi_b200_decompress(const void* codes, int64_t code_pitch, const void* ex
   const char* fn = "optimi_b200_decompress";
   int rc = check_shape(fn, rows, cols, dtype);
   if (rc != OPTIMI_OK || rows == 0 || cols == 0) return rc;
-  if (!out) return fail(OPTIMI_ERR_INVALID_ARGUMENT, "%s: out is NULL", fn);
+  if (!out || !aligned(out, 16)) return fail(OPTIMI_ERR_INVALID_ARGUMENT, "%s: out is NULL or not 16-byte aligned", fn);
   rc = check_codes(fn, codes, code_pitch, exponents, exponent_pitch, cols);
   if (rc == OPTIMI_OK) rc = check_items(fn, rows, cols);
   if (rc != OPTIMI_OK) return rc;
-  FOR_DTYPE(dtype, {
-    constexpr int V = 16 / (int)sizeof(T);
-    if (cols % V == 0 && aligned(out, 16))
-      launch_decompress<T, V>(codes, code_pitch, exponents, exponent_pitch, channel_scale, rows, cols, out, (cudaStream_t)stream);
-    else
-      launch_decompress<T, 1>(codes, code_pitch, exponents, exponent_pitch, channel_scale, rows, cols, out, (cudaStream_t)stream);
-  });
+  cudaStream_t s = (cudaStream_t)stream;
+  if (channel_scale)
+    FOR_DTYPE(dtype, launch_decompress<T, true>(codes, code_pitch, exponents, exponent_pitch, channel_scale, rows, cols, out, s));
+  else
+    FOR_DTYPE(dtype, launch_decompress<T, false>(codes, code_pitch, exponents, exponent_pitch, nullptr, rows, cols, out, s));
   return launched(fn);
 }
 
@@ -576,26 +686,27 @@ int optimi_b200_rms_norm(const void* x, int64_t x_stride, const void* residual, 
   }
   cudaStream_t s = (cudaStream_t)stream;
   const int size = dtype == OPTIMI_F32 ? 4 : 2;
-  const bool vectors = rows_aligned(x, x_stride, rows, size) && (!residual || rows_aligned(residual, residual_stride, rows, size)) &&
-                       (!weight || aligned(weight, 16)) && aligned(y, 16) && (!sum || aligned(sum, 16));
-  const Deal d = deal_of(cols, size, vectors);
+  const bool any = cols * size % 16 || !rows_aligned(x, x_stride, rows, size) || (residual && !rows_aligned(residual, residual_stride, rows, size)) ||
+                   !aligned(weight, 16) || !aligned(y, 16) || !aligned(sum, 16);
+  const Deal d = deal_of(cols, size, any ? kForwardAnyChunks : kForwardChunks);
   FOR_DTYPE(dtype, {
     if (d.K == 0) {
       long_rms_norm_kernel<T><<<grid_of(rows, 1 << 20), 512, 0, s>>>((const T*)x, x_stride, (const T*)residual, residual_stride, (const T*)weight,
                                                                     rows, cols, eps, (T*)y, (T*)sum, (int8_t*)codes, code_pitch,
                                                                     (uint8_t*)exponents, exponent_pitch, rstd);
     } else {
-      with_deal<T>(d, [&](auto c, auto p, auto k) {
-        constexpr int C = decltype(c)::value, P = decltype(p)::value, K = decltype(k)::value, kThreads = P < 128 ? 128 : P;
+      const auto with_constants = [&](auto p, auto k, auto is_any) {
+        constexpr int P = decltype(p)::value, K = decltype(k)::value, kThreads = P < 128 ? 128 : P;
+        constexpr bool kIsAny = decltype(is_any)::value;
         const unsigned blocks = grid_of((rows + kThreads / P - 1) / (kThreads / P), 1 << 20);
-        if (keep)
-          rms_norm_kernel<T, C, P, K, true><<<blocks, kThreads, 0, s>>>((const T*)x, x_stride, (const T*)residual, residual_stride, (const T*)weight,
-                                                                       rows, (int)cols, eps, (T*)y, (T*)sum, (int8_t*)codes, code_pitch,
-                                                                       (uint8_t*)exponents, exponent_pitch, rstd);
-        else
-          rms_norm_kernel<T, C, P, K, false><<<blocks, kThreads, 0, s>>>((const T*)x, x_stride, (const T*)residual, residual_stride, (const T*)weight,
-                                                                        rows, (int)cols, eps, (T*)y, (T*)sum, nullptr, 0, nullptr, 0, nullptr);
-      });
+        const auto launch = [&](auto kernel) {
+          kernel<<<blocks, kThreads, 0, s>>>((const T*)x, x_stride, (const T*)residual, residual_stride, (const T*)weight, rows, (int)cols, eps,
+                                             (T*)y, (T*)sum, (int8_t*)codes, code_pitch, (uint8_t*)exponents, exponent_pitch, rstd);
+        };
+        keep ? launch(rms_norm_kernel<T, P, K, kIsAny, true>) : launch(rms_norm_kernel<T, P, K, kIsAny, false>);
+      };
+      if (any) with_deal<T, kForwardAnyChunks>(d, [&](auto p, auto k) { with_constants(p, k, std::true_type()); });
+      else with_deal<T, kForwardChunks>(d, [&](auto p, auto k) { with_constants(p, k, std::false_type()); });
     }
   });
   return launched(fn);
@@ -631,26 +742,26 @@ int optimi_b200_rms_norm_backward(const void* grad, int64_t grad_stride, const v
   if (grad_weight && (!workspace || workspace_bytes < need))
     return fail(OPTIMI_ERR_WORKSPACE_TOO_SMALL, "%s: workspace has %zu bytes, %zu are needed", fn, workspace ? workspace_bytes : (size_t)0, need);
   const int size = dtype == OPTIMI_F32 ? 4 : 2;
-  const bool vectors = rows_aligned(grad, grad_stride, rows, size) && (!grad_sum || rows_aligned(grad_sum, grad_sum_stride, rows, size)) &&
-                       (!weight || aligned(weight, 16)) && (!grad_input || aligned(grad_input, 16));
-  const Deal d = deal_of(cols, size, vectors);
+  const bool any = cols * size % 16 || !rows_aligned(grad, grad_stride, rows, size) || (grad_sum && !rows_aligned(grad_sum, grad_sum_stride, rows, size)) ||
+                   !aligned(weight, 16) || !aligned(grad_input, 16);
+  const Deal d = deal_of(cols, size, kBackwardChunks);
   float* lines = grad_weight ? (float*)workspace : nullptr;
   unsigned blocks = 0;
   FOR_DTYPE(dtype, {
-    if (d.K == 0 || d.P > 512) {
+    if (d.K == 0) {
       blocks = backward_blocks(rows);
       long_rms_norm_backward_kernel<T><<<blocks, 512, 0, s>>>((const T*)grad, grad_stride, (const T*)grad_sum, grad_sum_stride, (const int8_t*)codes,
                                                               code_pitch, (const uint8_t*)exponents, exponent_pitch, rstd, (const T*)weight,
                                                               rows, cols, (T*)grad_input, lines);
     } else {
-      with_deal<T>(d, [&](auto c, auto p, auto k) {
-        constexpr int C = decltype(c)::value, P = decltype(p)::value, K = decltype(k)::value, kThreads = 512;
-        if constexpr (P <= 512) {
-          blocks = grid_of((rows + kThreads / P - 1) / (kThreads / P), kBackwardBlocks);
-          rms_norm_backward_kernel<T, C, P, K, kThreads><<<blocks, kThreads, kThreads > P ? (size_t)cols * sizeof(float) : 0, s>>>(
-              (const T*)grad, grad_stride, (const T*)grad_sum, grad_sum_stride, (const int8_t*)codes, code_pitch, (const uint8_t*)exponents,
-              exponent_pitch, rstd, (const T*)weight, rows, (int)cols, (T*)grad_input, lines);
-        }
+      with_deal<T, kBackwardChunks>(d, [&](auto p, auto k) {
+        constexpr int P = decltype(p)::value, K = decltype(k)::value;
+        blocks = grid_of((rows + 512 / P - 1) / (512 / P), kBackwardBlocks);
+        const auto launch = [&](auto kernel) {
+          kernel<<<blocks, 512, 0, s>>>((const T*)grad, grad_stride, (const T*)grad_sum, grad_sum_stride, (const int8_t*)codes, code_pitch,
+                                        (const uint8_t*)exponents, exponent_pitch, rstd, (const T*)weight, rows, (int)cols, (T*)grad_input, lines);
+        };
+        any ? launch(rms_norm_backward_kernel<T, P, K, true>) : launch(rms_norm_backward_kernel<T, P, K, false>);
       });
     }
   });
