@@ -319,10 +319,13 @@ int optimi_b200_rms_norm_backward(const void* grad, int64_t grad_stride, const v
  * sum over t of grad[t][o] * X[t][c], rounded once (`channel_scale` NULL: 1).  dtype (of grad,
  * channel_scale and grad_weight): OPTIMI_BF16 or OPTIMI_F16.  `workspace`: DEVICE scratch of
  * optimi_b200_weight_gradient_workspace_bytes(rows, outputs, channels) bytes, 16-byte aligned.  Rows of grad
- * begin on 16 bytes (grad_stride a multiple of 8).
+ * begin on 16 bytes (grad_stride a multiple of 8); optimi_b200_align_rows copies rows that do not to rows that do
+ * (out_stride: cols rounded up to 16 bytes; zeros behind a row).
  * optimi_b200_weight_gradient_status: *gave_up (HOST) is nonzero if a wait inside a kernel of the current
  * device ever ran out (a defect: that call's results are NaN).  Waits for the device. */
 int optimi_b200_weight_gradient_status(int* gave_up);
+int optimi_b200_align_rows(const void* x, int64_t x_stride, int64_t rows, int64_t cols, int dtype, void* out, int64_t out_stride,
+                           void* stream);
 size_t optimi_b200_weight_gradient_workspace_bytes(int64_t rows, int64_t outputs, int64_t channels);
 int optimi_b200_weight_gradient(const void* grad, int64_t grad_stride, const void* codes, int64_t code_pitch,
                                 const void* exponents, int64_t exponent_pitch, const void* channel_scale, int64_t rows,

@@ -39,6 +39,7 @@ ACTIVATION_SIGNATURES = {
     "optimi_b200_rms_norm": [_P, _L, _P, _L, _P, _L, _L, _D, _I, _P, _P, _P, _L, _P, _L, _P, _P],
     "optimi_b200_rms_norm_backward": [_P, _L, _P, _L, _P, _L, _P, _L, _P, _P, _L, _L, _I, _P, _P, _P, _Z, _P],
     "optimi_b200_weight_gradient_status": [_P],
+    "optimi_b200_align_rows": [_P, _L, _L, _L, _I, _P, _L, _P],
     "optimi_b200_weight_gradient": [_P, _L, _P, _L, _P, _L, _P, _L, _L, _L, _I, _P, _P, _Z, _P],
 }
 SIGNATURES.update(ACTIVATION_SIGNATURES)

@@ -247,17 +247,23 @@ def weight_gradient(grad: Tensor, saved: CompressedActivation) -> Tensor:
     m = _as_rows(grad.detach())
     rows, outputs = m.shape
     channels = saved.shape[-1]
-    if m.data_ptr() % 16 or rows > 1 and m.stride(0) % 8 or rows == 1 and outputs % 8:  # the copy engine loads from multiples of 16 bytes
-        m = torch.empty((rows, -(-outputs // 8) * 8), dtype=grad.dtype, device=grad.device)[:, :outputs].copy_(m)
-    stride = m.stride(0) if rows > 1 else -(-outputs // 8) * 8
-    dw = torch.empty((outputs, channels), dtype=grad.dtype, device=grad.device)
+    device, code = grad.device, _lib.DTYPE_CODE[grad.dtype]
+    pitch = -(-outputs // 8) * 8
+    copied = m.data_ptr() % 16 != 0 or (m.stride(0) if rows > 1 else outputs) % 8 != 0  # the kernel loads rows that begin on 16 bytes
+    stride = pitch if copied or rows <= 1 else m.stride(0)
+    dw = torch.empty((outputs, channels), dtype=grad.dtype, device=device)
     scale = None if saved.channel_scale is None else saved.channel_scale.detach().contiguous()
     need = _lib.LIB.optimi_b200_weight_gradient_workspace_bytes(rows, outputs, channels)
-    workspace = torch.empty(need, dtype=torch.uint8, device=grad.device) if need else None
-    with _on_device(grad.device):
+    workspace = torch.empty(need, dtype=torch.uint8, device=device) if need else None
+    with _on_device(device):
+        stream = _stream(device)
+        if copied:
+            source, m = m, torch.empty((rows, pitch), dtype=grad.dtype, device=device)
+            _lib.check(_lib.LIB.optimi_b200_align_rows(
+                source.data_ptr(), source.stride(0), rows, outputs, code, m.data_ptr(), pitch, stream))  # fmt: skip
         _lib.check(_lib.LIB.optimi_b200_weight_gradient(
-            m.data_ptr(), stride, *saved._layout(), _ptr(scale), rows, outputs, channels, _lib.DTYPE_CODE[grad.dtype], dw.data_ptr(),
-            _ptr(workspace), need, _stream(grad.device)))  # fmt: skip
+            m.data_ptr(), stride, *saved._layout(), _ptr(scale), rows, outputs, channels, code, dw.data_ptr(), _ptr(workspace),
+            need, stream))  # fmt: skip
     return dw
 
 

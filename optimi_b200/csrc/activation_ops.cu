@@ -103,7 +103,31 @@ __global__ void __launch_bounds__(kBlock) decompress_kernel(const int8_t* __rest
   }
 }
 
-// The same for rows that begin anywhere.  The result has no gaps, so an item is one 16-byte block of it as a whole; its codes lie at
+// Rows that begin anywhere, copied to rows that begin on 16 bytes (zeros up to the pitch): the tensor copy engine, which feeds the
+// weight gradient, loads nothing else.
+template <typename T>
+__global__ void __launch_bounds__(kBlock) align_rows_kernel(const T* __restrict__ x, int64_t items, int64_t chunks, int64_t cols, int64_t stride,
+                                                            T* __restrict__ out) {
+  constexpr int C = Chunk<T>::C;
+  const int64_t first = (int64_t)blockIdx.x * (kBlock * kUnroll) + threadIdx.x;
+  Fetched<T, true> in[kUnroll];
+  const T* from[kUnroll];
+  int n[kUnroll];
+#pragma unroll
+  for (int u = 0; u < kUnroll; u++) {
+    const int64_t item = first + u * kBlock;
+    int64_t row, col;
+    divide(item, chunks, &row, &col);
+    from[u] = x + row * stride + col * C;
+    n[u] = item < items ? (int)min((int64_t)C, cols - col * C) : 0;
+    in[u].fetch(from[u], n[u]);
+  }
+#pragma unroll
+  for (int u = 0; u < kUnroll; u++)
+    if (first + u * kBlock < items) in[u].settle(from[u], n[u]).store(out + (first + u * kBlock) * C);
+}
+
+// decompress for rows that begin anywhere.  The result has no gaps, so an item is one 16-byte block of it as a whole; its codes lie at
 // any byte of a row (whose pitch is a multiple of 32), and a block that reaches into the next row takes them one by one.
 template <typename T, bool kScaled>
 __global__ void __launch_bounds__(kBlock) decompress_any_kernel(const int8_t* __restrict__ codes, int64_t pitch, const uint8_t* __restrict__ exponents,
@@ -666,6 +690,22 @@ int optimi_b200_decompress(const void* codes, int64_t code_pitch, const void* ex
     FOR_DTYPE(dtype, launch_decompress<T, true>(codes, code_pitch, exponents, exponent_pitch, channel_scale, rows, cols, out, s));
   else
     FOR_DTYPE(dtype, launch_decompress<T, false>(codes, code_pitch, exponents, exponent_pitch, nullptr, rows, cols, out, s));
+  return launched(fn);
+}
+
+int optimi_b200_align_rows(const void* x, int64_t x_stride, int64_t rows, int64_t cols, int dtype, void* out, int64_t out_stride, void* stream) {
+  const char* fn = "optimi_b200_align_rows";
+  int rc = check_shape(fn, rows, cols, dtype);
+  if (rc != OPTIMI_OK || rows == 0 || cols == 0) return rc;
+  const int64_t values = dtype == OPTIMI_F32 ? 4 : 8, chunks = (cols + values - 1) / values;
+  if (!x || !out || !aligned(out, 16)) return fail(OPTIMI_ERR_INVALID_ARGUMENT, "%s: x or out is NULL, or out is not 16-byte aligned", fn);
+  if (out_stride != chunks * values)
+    return fail(OPTIMI_ERR_INVALID_ARGUMENT, "%s: out_stride is %lld, not %lld (cols up to the next 16 bytes)", fn, (long long)out_stride,
+                (long long)(chunks * values));
+  rc = check_items(fn, rows, cols);
+  if (rc != OPTIMI_OK) return rc;
+  const unsigned blocks = (unsigned)((rows * chunks + kBlock * kUnroll - 1) / (kBlock * kUnroll));
+  FOR_DTYPE(dtype, (align_rows_kernel<T><<<blocks, kBlock, 0, (cudaStream_t)stream>>>((const T*)x, rows * chunks, chunks, cols, x_stride, (T*)out)));
   return launched(fn);
 }
 

@@ -101,6 +101,10 @@ def test_entry_points_reject_bad_arguments_without_launching():
     refused(L.optimi_b200_weight_gradient(*with_(dw, _1=68)), b"begin on 16 bytes")
     refused(L.optimi_b200_weight_gradient(*with_(dw, _1=56)), b"begin on 16 bytes")
     refused(L.optimi_b200_weight_gradient_status(None), b"gave_up is NULL")
+    refused(L.optimi_b200_align_rows(p, 65, 4, 65, 1, p, 65, None), b"out_stride")
+    refused(L.optimi_b200_align_rows(p, 65, 4, 65, 1, odd, 72, None), b"not 16-byte aligned")
+    refused(L.optimi_b200_align_rows(None, 65, 4, 65, 1, p, 72, None), b"x or out is NULL")
+    refused(L.optimi_b200_align_rows(p, 65, 4, 65, 5, p, 72, None), b"dtype")
     # nothing to do is not an error
     assert L.optimi_b200_compress(None, 0, 0, 64, 1, None, 0, None, 0, None) == 0
     assert L.optimi_b200_rms_norm(*with_(norm, _5=0)) == 0
