@@ -178,21 +178,20 @@ def _stream(device: torch.device) -> int:
     return torch._C._cuda_getCurrentRawStream(device.index)
 
 
-class _on_device:
-    """`torch.cuda.device`, at no cost where that device is current already."""
+def _call(fn, device: torch.device, *args) -> None:
+    """Calls entry point `fn` with `args` and the current stream of `device`, that device being current."""
+    if torch.cuda.current_device() == device.index:
+        rc = fn(*args, _stream(device))
+    else:
+        with torch.cuda.device(device):
+            rc = fn(*args, _stream(device))
+    if rc:
+        _lib.check(rc)
 
-    __slots__ = ("guard",)
 
-    def __init__(self, device: torch.device):
-        self.guard = None if torch.cuda.current_device() == device.index else torch.cuda.device(device)
-
-    def __enter__(self):
-        if self.guard is not None:
-            self.guard.__enter__()
-
-    def __exit__(self, *exc):
-        if self.guard is not None:
-            self.guard.__exit__(*exc)
+def _dense_like(t: Tensor) -> Tensor:
+    """A new contiguous tensor of `t`'s shape and type."""
+    return torch.empty_like(t) if t.is_contiguous() else torch.empty(t.shape, dtype=t.dtype, device=t.device)
 
 
 def _buffer_bytes(rows: int, cols: int) -> tuple[int, int]:
@@ -210,9 +209,7 @@ def compress(x: Tensor) -> CompressedActivation:
     rows, cols = m.shape
     device = x.device
     saved = CompressedActivation._of((torch.empty(_buffer_bytes(rows, cols)[0], dtype=torch.uint8, device=device),), x.shape, x.dtype)
-    with _on_device(device):
-        _lib.check(_lib.LIB.optimi_b200_compress(
-            m.data_ptr(), m.stride(0), rows, cols, _lib.DTYPE_CODE[x.dtype], *saved._layout(), _stream(device)))  # fmt: skip
+    _call(_lib.LIB.optimi_b200_compress, device, m.data_ptr(), m.stride(0), rows, cols, _lib.DTYPE_CODE[x.dtype], *saved._layout())
     return saved
 
 
@@ -223,10 +220,8 @@ def decompress(saved: CompressedActivation) -> Tensor:
         raise RuntimeError(f"decompress: `saved` lives on {device}; optimi_b200 takes CUDA tensors only (there is no CPU path)")
     out = torch.empty(saved.shape, dtype=saved.dtype, device=device)
     scale = None if saved.channel_scale is None else saved.channel_scale.detach().contiguous()
-    with _on_device(device):
-        _lib.check(_lib.LIB.optimi_b200_decompress(
-            *saved._layout(), _ptr(scale), _rows(saved.shape), saved.shape[-1], _lib.DTYPE_CODE[saved.dtype], out.data_ptr(),
-            _stream(device)))  # fmt: skip
+    _call(_lib.LIB.optimi_b200_decompress, device, *saved._layout(), _ptr(scale), _rows(saved.shape), saved.shape[-1],
+          _lib.DTYPE_CODE[saved.dtype], out.data_ptr())  # fmt: skip
     return out
 
 
@@ -255,15 +250,11 @@ def weight_gradient(grad: Tensor, saved: CompressedActivation) -> Tensor:
     scale = None if saved.channel_scale is None else saved.channel_scale.detach().contiguous()
     need = _lib.LIB.optimi_b200_weight_gradient_workspace_bytes(rows, outputs, channels)
     workspace = torch.empty(need, dtype=torch.uint8, device=device) if need else None
-    with _on_device(device):
-        stream = _stream(device)
-        if copied:
-            source, m = m, torch.empty((rows, pitch), dtype=grad.dtype, device=device)
-            _lib.check(_lib.LIB.optimi_b200_align_rows(
-                source.data_ptr(), source.stride(0), rows, outputs, code, m.data_ptr(), pitch, stream))  # fmt: skip
-        _lib.check(_lib.LIB.optimi_b200_weight_gradient(
-            m.data_ptr(), stride, *saved._layout(), _ptr(scale), rows, outputs, channels, code, dw.data_ptr(), _ptr(workspace),
-            need, stream))  # fmt: skip
+    if copied:
+        source, m = m, torch.empty((rows, pitch), dtype=grad.dtype, device=device)
+        _call(_lib.LIB.optimi_b200_align_rows, device, source.data_ptr(), source.stride(0), rows, outputs, code, m.data_ptr(), pitch)
+    _call(_lib.LIB.optimi_b200_weight_gradient, device, m.data_ptr(), stride, *saved._layout(), _ptr(scale), rows, outputs, channels,
+          code, dw.data_ptr(), _ptr(workspace), need)  # fmt: skip
     return dw
 
 
@@ -273,19 +264,17 @@ def _norm_forward(x: Tensor, weight: Tensor | None, residual: Tensor | None, eps
     r = None if residual is None else _as_rows(residual)
     rows, cols = m.shape
     device = x.device
-    y = torch.empty(x.shape, dtype=x.dtype, device=device)
-    h = None if r is None else torch.empty(x.shape, dtype=x.dtype, device=device)
-    buffer = rstd = None
-    layout = (None, 0, None, 0)
+    y = _dense_like(x)
+    h = None if r is None else _dense_like(x)
+    buffer = None
+    kept = (None, 0, None, 0, None)
     if keep:
         _, after = _buffer_bytes(rows, cols)
         buffer = torch.empty(after + 4 * rows, dtype=torch.uint8, device=device)
-        layout = CompressedActivation._of((buffer,), x.shape, x.dtype)._layout()
-        rstd = buffer.data_ptr() + after
-    with _on_device(device):
-        _lib.check(_lib.LIB.optimi_b200_rms_norm(
-            m.data_ptr(), m.stride(0), _ptr(r), 0 if r is None else r.stride(0), _ptr(weight), rows, cols, eps,
-            _lib.DTYPE_CODE[x.dtype], y.data_ptr(), _ptr(h), *layout, rstd, _stream(device)))  # fmt: skip
+        at, groups = buffer.data_ptr(), -(-cols // GROUP)
+        kept = (at, groups * GROUP, at + rows * groups * GROUP, groups, at + after)
+    _call(_lib.LIB.optimi_b200_rms_norm, device, m.data_ptr(), m.stride(0), _ptr(r), 0 if r is None else r.stride(0), _ptr(weight),
+          rows, cols, eps, _lib.DTYPE_CODE[x.dtype], y.data_ptr(), _ptr(h), *kept)  # fmt: skip
     return y, h, buffer
 
 
@@ -311,15 +300,14 @@ class _RMSNorm(torch.autograd.Function):
         s = None if grad_sum is None else _as_rows(grad_sum)
         w = None if weight is None else weight.contiguous()
         rows, cols = g.shape
-        dx = torch.empty(grad.shape, dtype=grad.dtype, device=grad.device) if need_x or need_r else None
+        dx = _dense_like(grad) if need_x or need_r else None
         dw = torch.empty_like(w) if need_w else None
         need = _lib.LIB.optimi_b200_rms_norm_backward_workspace_bytes(rows, cols) if need_w else 0
         workspace = torch.empty(need, dtype=torch.uint8, device=grad.device) if need else None
-        with _on_device(grad.device):
-            _lib.check(_lib.LIB.optimi_b200_rms_norm_backward(
-                g.data_ptr(), g.stride(0), _ptr(s), 0 if s is None else s.stride(0),
-                *CompressedActivation._of((buffer,), grad.shape, grad.dtype)._layout(), buffer.data_ptr() + _buffer_bytes(rows, cols)[1],
-                _ptr(w), rows, cols, _lib.DTYPE_CODE[grad.dtype], _ptr(dx), _ptr(dw), _ptr(workspace), need, _stream(grad.device)))  # fmt: skip
+        at, groups = buffer.data_ptr(), -(-cols // GROUP)
+        _call(_lib.LIB.optimi_b200_rms_norm_backward, grad.device, g.data_ptr(), g.stride(0), _ptr(s), 0 if s is None else s.stride(0),
+              at, groups * GROUP, at + rows * groups * GROUP, groups, at + _buffer_bytes(rows, cols)[1], _ptr(w), rows, cols,
+              _lib.DTYPE_CODE[grad.dtype], _ptr(dx), _ptr(dw), _ptr(workspace), need)  # fmt: skip
         return dx if need_x else None, dw, dx if need_r else None, None, None
 
 

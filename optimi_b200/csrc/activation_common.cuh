@@ -158,37 +158,58 @@ struct Chunk {
       return;
     }
     const int lane = threadIdx.x % 32, head = (16 - (int)off) / (int)sizeof(T);  // values of a chunk that lie in its first block
-    Chunk before;
+    const uint32_t skip = 16 - off;                                                // their bytes
+    uint32_t u[8];
 #pragma unroll
-    for (int i = 0; i < 4; i++) before.w[i] = __shfl_up_sync(~0u, w[i], 1);
+    for (int i = 0; i < 4; i++) u[i] = __shfl_up_sync(~0u, w[i], 1), u[4 + i] = w[i];
     const int n_before = __shfl_up_sync(~0u, n, 1);
-    if (lane > 0 && n >= head) {  // then the chunk before is whole
-      uint32_t u[8] = {before.w[0], before.w[1], before.w[2], before.w[3], w[0], w[1], w[2], w[3]};
-      // the block is bytes 16 - off .. 31 - off of the two
-      const uint32_t skip = 16 - off;
-      if (skip & 8) {
-#pragma unroll
-        for (int i = 0; i < 6; i++) u[i] = u[i + 2];
-      }
-      if (skip & 4) {
-#pragma unroll
-        for (int i = 0; i < 5; i++) u[i] = u[i + 1];
-      }
-      Chunk out;
-#pragma unroll
-      for (int i = 0; i < 4; i++) out.w[i] = sizeof(T) == 2 ? __funnelshift_r(u[i], u[i + 1], (skip & 2) * 8) : u[i];
-      out.store(reinterpret_cast<T*>(reinterpret_cast<uintptr_t>(p) - off));
+    if (lane > 0 && n >= head) {  // then the chunk before is whole, and the block is bytes skip .. skip + 15 of the two
+      shift(u, skip);
+      *reinterpret_cast<uint4*>(reinterpret_cast<uintptr_t>(p) - off) = make_uint4(u[0], u[1], u[2], u[3]);
+    } else if (lane == 0 && n == C) {  // the head alone, up to the next block: 2, 4 and 8 bytes of it
+      uint32_t a[8] = {w[0], w[1], w[2], w[3], 0, 0, 0, 0};
+      char* at = reinterpret_cast<char*>(p);
+      if (sizeof(T) == 2 && (skip & 2)) *reinterpret_cast<unsigned short*>(at) = (unsigned short)a[0], at += 2, shift(a, 2);
+      if (skip & 4) *reinterpret_cast<uint32_t*>(at) = a[0], at += 4, shift(a, 4);
+      if (skip & 8) *reinterpret_cast<uint2*>(at) = make_uint2(a[0], a[1]);
     } else {
+      Chunk before;
+#pragma unroll
+      for (int i = 0; i < 4; i++) before.w[i] = u[i];
 #pragma unroll
       for (int i = 0; i < C; i++) {
         if (lane > 0 && i >= head && i < n_before) before.store_value(p - C, i);
         if (i < head && i < n) store_value(p, i);
       }
     }
-    if (lane == 31) {
+    if (lane == 31 && n > head) {  // the tail, which no lane after this one takes along
+      if (n == C) {
+        uint32_t a[8] = {w[0], w[1], w[2], w[3], 0, 0, 0, 0};
+        shift(a, skip);
+        char* at = reinterpret_cast<char*>(reinterpret_cast<uintptr_t>(p) + skip);
+        if (off & 8) *reinterpret_cast<uint2*>(at) = make_uint2(a[0], a[1]), at += 8, shift(a, 8);
+        if (off & 4) *reinterpret_cast<uint32_t*>(at) = a[0], at += 4, shift(a, 4);
+        if (sizeof(T) == 2 && (off & 2)) *reinterpret_cast<unsigned short*>(at) = (unsigned short)a[0];
+      } else {
 #pragma unroll
-      for (int i = 0; i < C; i++)
-        if (i >= head && i < n) store_value(p, i);
+        for (int i = 0; i < C; i++)
+          if (i >= head && i < n) store_value(p, i);
+      }
+    }
+  }
+  // The first 16 of 32 bytes, from byte `by` (below 16) on.
+  static __device__ __forceinline__ void shift(uint32_t (&u)[8], uint32_t by) {
+    if (by & 8) {
+#pragma unroll
+      for (int i = 0; i < 6; i++) u[i] = u[i + 2];
+    }
+    if (by & 4) {
+#pragma unroll
+      for (int i = 0; i < 5; i++) u[i] = u[i + 1];
+    }
+    if constexpr (sizeof(T) == 2) {
+#pragma unroll
+      for (int i = 0; i < 4; i++) u[i] = __funnelshift_r(u[i], u[i + 1], (by & 2) * 8);
     }
   }
 
@@ -249,20 +270,12 @@ struct Fetched {
 #pragma unroll
       for (int i = 0; i < 4; i++) v.w[i] = u[i];
     } else {
-      const uint32_t off = (uint32_t)reinterpret_cast<uintptr_t>(p) & 15u;
       uint32_t s[8];
 #pragma unroll
       for (int i = 0; i < 8; i++) s[i] = u[i];
-      if (off & 8) {
+      Chunk<T>::shift(s, (uint32_t)reinterpret_cast<uintptr_t>(p) & 15u);
 #pragma unroll
-        for (int i = 0; i < 6; i++) s[i] = s[i + 2];
-      }
-      if (off & 4) {
-#pragma unroll
-        for (int i = 0; i < 5; i++) s[i] = s[i + 1];
-      }
-#pragma unroll
-      for (int i = 0; i < 4; i++) v.w[i] = sizeof(T) == 2 ? __funnelshift_r(s[i], s[i + 1], (off & 2) * 8) : s[i];
+      for (int i = 0; i < 4; i++) v.w[i] = s[i];
       if (n < C) {
 #pragma unroll
         for (int i = 0; i < 4; i++) {

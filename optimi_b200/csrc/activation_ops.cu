@@ -565,8 +565,9 @@ static bool rows_aligned(const void* p, int64_t stride, int64_t rows, int size) 
 
 // How a row is dealt out: P threads with K chunks each, K at most `most` as long as 512 threads are enough.  K = 0: too long for
 // registers.  16384 x 4096 bf16, K = 1, 2, 4: forward 141, 108, 100 us; backward 113, 90, 136 us (for 4 there are no registers to
-// ask ahead); forward with rows that begin anywhere, 4096 x 4095: 59, 51, 61 us.
-constexpr int kForwardChunks = 4, kForwardAnyChunks = 2, kBackwardChunks = 2;
+// ask ahead); rows that begin anywhere,
+// 4096 x 4095: forward 59, 51, 61 us, backward 60, 77 us (two chunks and the next row's two do not fit into registers).
+constexpr int kForwardChunks = 4, kForwardAnyChunks = 2, kBackwardChunks = 2, kBackwardAnyChunks = 1;
 
 struct Deal {
   int P, K;
@@ -784,7 +785,7 @@ int optimi_b200_rms_norm_backward(const void* grad, int64_t grad_stride, const v
   const int size = dtype == OPTIMI_F32 ? 4 : 2;
   const bool any = cols * size % 16 || !rows_aligned(grad, grad_stride, rows, size) || (grad_sum && !rows_aligned(grad_sum, grad_sum_stride, rows, size)) ||
                    !aligned(weight, 16) || !aligned(grad_input, 16);
-  const Deal d = deal_of(cols, size, kBackwardChunks);
+  const Deal d = deal_of(cols, size, any ? kBackwardAnyChunks : kBackwardChunks);
   float* lines = grad_weight ? (float*)workspace : nullptr;
   unsigned blocks = 0;
   FOR_DTYPE(dtype, {
@@ -794,15 +795,16 @@ int optimi_b200_rms_norm_backward(const void* grad, int64_t grad_stride, const v
                                                               code_pitch, (const uint8_t*)exponents, exponent_pitch, rstd, (const T*)weight,
                                                               rows, cols, (T*)grad_input, lines);
     } else {
-      with_deal<T, kBackwardChunks>(d, [&](auto p, auto k) {
+      const auto with_constants = [&](auto p, auto k, auto is_any) {
         constexpr int P = decltype(p)::value, K = decltype(k)::value;
+        constexpr bool kIsAny = decltype(is_any)::value;
         blocks = grid_of((rows + 512 / P - 1) / (512 / P), kBackwardBlocks);
-        const auto launch = [&](auto kernel) {
-          kernel<<<blocks, 512, 0, s>>>((const T*)grad, grad_stride, (const T*)grad_sum, grad_sum_stride, (const int8_t*)codes, code_pitch,
-                                        (const uint8_t*)exponents, exponent_pitch, rstd, (const T*)weight, rows, (int)cols, (T*)grad_input, lines);
-        };
-        any ? launch(rms_norm_backward_kernel<T, P, K, true>) : launch(rms_norm_backward_kernel<T, P, K, false>);
-      });
+        rms_norm_backward_kernel<T, P, K, kIsAny><<<blocks, 512, 0, s>>>(
+            (const T*)grad, grad_stride, (const T*)grad_sum, grad_sum_stride, (const int8_t*)codes, code_pitch, (const uint8_t*)exponents,
+            exponent_pitch, rstd, (const T*)weight, rows, (int)cols, (T*)grad_input, lines);
+      };
+      if (any) with_deal<T, kBackwardAnyChunks>(d, [&](auto p, auto k) { with_constants(p, k, std::true_type()); });
+      else with_deal<T, kBackwardChunks>(d, [&](auto p, auto k) { with_constants(p, k, std::false_type()); });
     }
   });
   rc = launched(fn);
