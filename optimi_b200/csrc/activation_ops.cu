@@ -21,6 +21,20 @@ static __device__ __forceinline__ void divide(int64_t a, int64_t b, int64_t* quo
   }
 }
 
+// The rows and columns (in units of `per_row` a row) of the items that a thread takes: one division, then steps of kBlock items.
+struct Walk {
+  int64_t row, col;
+  int64_t rows_on, cols_on, per_row;
+  __device__ __forceinline__ Walk(int64_t item, int64_t step, int64_t units_per_row) : per_row(units_per_row) {
+    divide(item, per_row, &row, &col);
+    divide(step, per_row, &rows_on, &cols_on);
+  }
+  __device__ __forceinline__ void on() {
+    row += rows_on, col += cols_on;
+    if (col >= per_row) col -= per_row, row++;
+  }
+};
+
 // How the rows of the 16-bit or 32-bit tensor lie.  kFlat: whole groups, one row after another without a gap, so that it is one
 // long row and nothing is divided.  kRows: every row begins on 16 bytes and is whole chunks.  kAny: neither.
 enum Lie : int { kFlat, kRows, kAny };
@@ -34,12 +48,12 @@ __global__ void __launch_bounds__(kBlock) compress_kernel(const T* __restrict__ 
   Fetched<T, kLie == kAny> in[kUnroll];
   int64_t row[kUnroll], col[kUnroll];
   int n[kUnroll];
+  Walk walk(kLie == kFlat ? 0 : first, kBlock, kLie == kFlat ? 1 : chunks);
 #pragma unroll
   for (int u = 0; u < kUnroll; u++) {
     const int64_t item = first + u * kBlock;
-    row[u] = 0, col[u] = item;
-    if (kLie != kFlat) divide(item, chunks, &row[u], &col[u]);
-    col[u] *= C;
+    row[u] = kLie == kFlat ? 0 : walk.row, col[u] = (kLie == kFlat ? item : walk.col) * C;
+    if (kLie != kFlat) walk.on();
     n[u] = item >= items ? 0 : kLie == kFlat ? C : (int)min((int64_t)C, cols - col[u]);
     in[u].fetch(x + row[u] * stride + col[u], n[u]);
   }
@@ -68,12 +82,12 @@ __global__ void __launch_bounds__(kBlock) decompress_kernel(const int8_t* __rest
   CodeChunk<C> c[kUnroll];
   uint32_t e[kUnroll];
   int64_t row[kUnroll], col[kUnroll];
+  Walk walk(kLie == kFlat ? 0 : first, kBlock, kLie == kFlat ? 1 : chunks);
 #pragma unroll
   for (int u = 0; u < kUnroll; u++) {
     const int64_t item = first + u * kBlock;
-    row[u] = 0, col[u] = item;
-    if (kLie != kFlat) divide(item, chunks, &row[u], &col[u]);
-    col[u] *= C;
+    row[u] = kLie == kFlat ? 0 : walk.row, col[u] = (kLie == kFlat ? item : walk.col) * C;
+    if (kLie != kFlat) walk.on();
     c[u].clear(), e[u] = 0;
     if (item < items) {
       c[u].load(codes + row[u] * pitch + col[u]);
@@ -113,13 +127,11 @@ __global__ void __launch_bounds__(kBlock) align_rows_kernel(const T* __restrict_
   Fetched<T, true> in[kUnroll];
   const T* from[kUnroll];
   int n[kUnroll];
+  Walk walk(first, kBlock, chunks);
 #pragma unroll
-  for (int u = 0; u < kUnroll; u++) {
-    const int64_t item = first + u * kBlock;
-    int64_t row, col;
-    divide(item, chunks, &row, &col);
-    from[u] = x + row * stride + col * C;
-    n[u] = item < items ? (int)min((int64_t)C, cols - col * C) : 0;
+  for (int u = 0; u < kUnroll; u++, walk.on()) {
+    from[u] = x + walk.row * stride + walk.col * C;
+    n[u] = first + u * kBlock < items ? (int)min((int64_t)C, cols - walk.col * C) : 0;
     in[u].fetch(from[u], n[u]);
   }
 #pragma unroll
@@ -135,28 +147,37 @@ __global__ void __launch_bounds__(kBlock) decompress_any_kernel(const int8_t* __
                                                                 int64_t cols, T* __restrict__ out) {
   constexpr int C = Chunk<T>::C;
   const int64_t first = (int64_t)blockIdx.x * (kBlock * kUnroll) + threadIdx.x;
+  uint32_t w[kUnroll][C / 4 + 1];
+  uint32_t low[kUnroll], high[kUnroll];
+  int64_t col[kUnroll];
+  Walk walk(first * C, kBlock * C, cols);
+#pragma unroll
+  for (int u = 0; u < kUnroll; u++, walk.on()) {
+    col[u] = walk.col;
+#pragma unroll
+    for (int i = 0; i <= C / 4; i++) w[u][i] = 0;
+    low[u] = high[u] = 0;
+    if ((first + u * kBlock) * C < values && walk.col + C <= cols) {
+      const uint32_t* words = reinterpret_cast<const uint32_t*>(codes + walk.row * pitch + (walk.col & ~3ll));
+#pragma unroll
+      for (int i = 0; i < C / 4; i++) w[u][i] = words[i];
+      if (walk.col & 3) w[u][C / 4] = words[C / 4];  // the last code asked for lies there
+      const uint8_t* group = exponents + walk.row * epitch + walk.col / kGroup;
+      low[u] = group[0], high[u] = group[((int)(walk.col % kGroup) + C - 1) / kGroup];
+    }
+  }
 #pragma unroll
   for (int u = 0; u < kUnroll; u++) {
     const int64_t at = (first + u * kBlock) * C;
     if (at >= values) return;
-    int64_t row, col;
-    divide(at, cols, &row, &col);
     float f[C];
-    if (col + C <= cols) {
-      const uint32_t* words = reinterpret_cast<const uint32_t*>(codes + row * pitch + (col & ~3ll));
-      const uint32_t shift = (uint32_t)(col & 3) * 8;
-      uint32_t w[C / 4 + 1];
-#pragma unroll
-      for (int i = 0; i < C / 4; i++) w[i] = words[i];
-      w[C / 4] = shift ? words[C / 4] : 0;  // the last code asked for lies there
+    if (col[u] + C <= cols) {
       CodeChunk<C> c;
 #pragma unroll
-      for (int i = 0; i < C / 4; i++) c.w[i] = __funnelshift_r(w[i], w[i + 1], shift);
-      const uint8_t* group = exponents + row * epitch + col / kGroup;
-      const int in = (int)(col % kGroup);
-      const float low = power_of(group[0]), high = power_of(group[(in + C - 1) / kGroup]);
+      for (int i = 0; i < C / 4; i++) c.w[i] = __funnelshift_r(w[u][i], w[u][i + 1], (uint32_t)(col[u] & 3) * 8);
+      const int in = (int)(col[u] % kGroup);
 #pragma unroll
-      for (int i = 0; i < C; i++) f[i] = __fmul_rn(c.get(i), in + i < kGroup ? low : high);
+      for (int i = 0; i < C; i++) f[i] = __fmul_rn(c.get(i), power_of((int)(in + i < kGroup ? low[u] : high[u])));
     } else {
 #pragma unroll
       for (int i = 0; i < C; i++) {
@@ -167,7 +188,7 @@ __global__ void __launch_bounds__(kBlock) decompress_any_kernel(const int8_t* __
     }
     if constexpr (kScaled) {
 #pragma unroll
-      for (int i = 0; i < C; i++) f[i] = __fmul_rn(f[i], to_f32(channel_scale[(col + i) % cols]));
+      for (int i = 0; i < C; i++) f[i] = __fmul_rn(f[i], to_f32(channel_scale[(col[u] + i) % cols]));
     }
     Chunk<T> v;
     v.set(f);
