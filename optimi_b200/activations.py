@@ -160,6 +160,8 @@ def _check(name: str, what: str, t: Tensor, like: Tensor | None = None) -> None:
 
 def _as_rows(t: Tensor) -> Tensor:
     """`t` as a matrix of its last dimension whose rows are contiguous and do not overlap: itself where that holds, else a copy."""
+    if t.is_neg():  # a lazily negated view: its memory holds the opposite
+        t = t.detach().resolve_neg()
     if t.dim() != 2:
         t = t.detach().reshape(_rows(t.shape), t.shape[-1])
     if t.is_contiguous():
@@ -447,9 +449,9 @@ def checkpoint(function: Callable, *args: Any, **kwargs: Any):
 
 
 def _kept(x: Tensor) -> CompressedActivation | None:
-    """The 8-bit form a norm attached to this very tensor, unless the tensor was written to since."""
+    """The 8-bit form a norm attached to this very tensor, unless the tensor was written to or given other memory since."""
     kept = getattr(x, _KEPT_ATTR, None)
-    return kept[0] if kept is not None and kept[1] == x._version else None
+    return kept[0] if kept is not None and kept[1:] == (x._version, x.data_ptr(), x.shape) else None
 
 
 class _CompressedLinear(nn.Linear):
@@ -469,8 +471,9 @@ class _CompressedRMSNorm(nn.RMSNorm):
         if torch.is_autocast_enabled("cuda") or (w is not None and w.dtype != x.dtype):
             return super().forward(x)
         out = rms_norm(x, w, eps=self.eps)
-        setattr(out.output, _KEPT_ATTR, (out.saved, out.output._version))
-        return out.output
+        y = out.output
+        setattr(y, _KEPT_ATTR, (out.saved, y._version, y.data_ptr(), y.shape))
+        return y
 
 
 def prepare_for_compressed_activations(model: nn.Module) -> nn.Module:

@@ -360,6 +360,8 @@ def check_weight_gradient(grad, saved, dw):
 WG_SHAPES = [  # tokens, outputs, channels
     (1, 1, 1), (1, 16, 16), (1, 512, 4096), (2, 8, 32), (7, 40, 72), (15, 100, 33), (16, 128, 128), (63, 129, 257), (64, 256, 256),
     (65, 255, 300), (128, 1000, 128), (512, 512, 128), (777, 1001, 96), (1000, 64, 2816), (4096, 256, 256), (9000, 72, 40), (300, 4096, 1024),
+    # tiles of 384 outputs, the last one 256 wide or less, whole turns and a cut one
+    (640, 9600, 1000), (200, 14336, 2048), (2048, 3900, 2900), (64, 6144, 3000), (130, 385, 257), (20000, 400, 130),
 ]  # fmt: skip
 
 
@@ -670,6 +672,118 @@ def test_a_norm_output_that_was_written_to_is_not_mistaken_for_the_kept_one():
     y.mul_(2)
     model[1](y).backward(dy)
     assert same_bits(model[1].weight.grad, act().weight_gradient(dy, act().compress(y.detach())))
+
+
+def test_a_norm_output_given_other_memory_is_not_mistaken_for_the_kept_one():
+    import optimi_b200
+
+    model = nn.Sequential(nn.RMSNorm(64), nn.Linear(64, 32, bias=False)).to(device="cuda", dtype=torch.bfloat16)
+    optimi_b200.prepare_for_compressed_activations(model)
+    x, dy = normal((40, 64), torch.bfloat16, 1).cuda(), normal((40, 32), torch.bfloat16, 2).cuda()
+    y = model[0](x)
+    y.data = y.data * 3
+    model[1](y).backward(dy)
+    assert same_bits(model[1].weight.grad, act().weight_gradient(dy, act().compress(y.detach())))
+
+
+def small_chain(dtype=torch.bfloat16):
+    a = act()
+    x, r = loud((50, 96), dtype, 1).cuda().requires_grad_(), normal((50, 96), dtype, 2).cuda().requires_grad_()
+    w = (1 + 0.1 * normal((96,), torch.float64, 9)).to(dtype).cuda().requires_grad_()
+    m = normal((40, 96), dtype, 3, 0.1).cuda().requires_grad_()
+    b = normal((40,), dtype, 4).cuda().requires_grad_()
+
+    def run():
+        out = a.rms_norm(x, w, r, eps=EPS)
+        return a.linear(out.output, m, b, saved=out.saved), out.residual
+
+    return [x, r, w, m, b], run, (normal((50, 40), dtype, 5, 0.1).cuda(), normal((50, 96), dtype, 6, 0.1).cuda())
+
+
+def test_leaf_gradients_are_tensors_of_their_own_and_accumulate():
+    leaves, run, grads = small_chain()
+    once = [g.clone() for g in torch.autograd.grad(run(), leaves, grads)]
+    for _ in range(2):
+        torch.autograd.backward(run(), grads)
+    assert len({t.grad.data_ptr() for t in leaves}) == len(leaves)
+    for t, g in zip(leaves, once):
+        assert same_bits(t.grad, g + g)
+
+
+def test_backward_twice_and_only_through_the_residual():
+    leaves, run, grads = small_chain()
+    outs = run()
+    first = torch.autograd.grad(outs, leaves, grads, retain_graph=True)
+    for a, b in zip(first, torch.autograd.grad(outs, leaves, grads)):
+        assert same_bits(a, b)
+    x, r, w, _, _ = leaves
+    gx, gr, gw = torch.autograd.grad(run()[1], (x, r, w), grads[1])
+    assert same_bits(gx, grads[1]) and same_bits(gr, grads[1]) and bool((gw == 0).all())
+
+
+def test_differentiating_a_gradient_is_refused():
+    leaves, run, grads = small_chain()
+    with pytest.raises(RuntimeError, match="create_graph"):
+        torch.autograd.grad(run(), leaves, grads, create_graph=True)
+    x = leaves[0]
+    with pytest.raises(RuntimeError, match="create_graph"):
+        torch.autograd.grad(act().rms_norm(x).output.sum(), x, create_graph=True)
+
+
+def test_what_is_kept_may_travel_through_saved_tensor_hooks():
+    leaves, run, grads = small_chain()
+    want = torch.autograd.grad(run(), leaves, grads)
+    with torch.autograd.graph.save_on_cpu():
+        outs = run()
+    for a, b in zip(torch.autograd.grad(outs, leaves, grads), want):
+        assert same_bits(a, b)
+
+
+def test_kept_rows_written_to_are_noticed():
+    a = act()
+    x = loud((50, 96), torch.bfloat16, 1).cuda().requires_grad_()
+    out = a.rms_norm(x)
+    out.saved.codes.zero_()
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        out.output.sum().backward()
+
+
+def test_lazily_negated_views():
+    a = act()
+    z = torch.complex(normal((6, 40), torch.float32, 1), normal((6, 40), torch.float32, 2)).cuda()
+    view = z.conj().imag
+    assert view.is_neg()
+    want = a.compress(view.clone())
+    got = a.compress(view)
+    assert torch.equal(got.codes, want.codes) and torch.equal(got.exponents, want.exponents)
+
+
+def test_calls_from_two_threads():
+    import threading
+
+    a = act()
+    x, dy = loud((300, 512), torch.bfloat16, 1).cuda(), normal((300, 128), torch.bfloat16, 2).cuda()
+    saved = a.compress(x)
+    want = a.weight_gradient(dy, saved)
+    torch.cuda.synchronize()
+    failures = []
+
+    def work():
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(50):
+                s = a.compress(x)
+                dw = a.weight_gradient(dy, s)
+                if not torch.equal(dw, want):
+                    failures.append("differs")
+                if a.rms_norm(x, eps=EPS).output.shape != x.shape:
+                    failures.append("shape")
+
+    threads = [threading.Thread(target=work) for _ in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failures
 
 
 def test_checkpoint_recomputes_from_eight_bits():
