@@ -304,12 +304,12 @@ int optimi_b200_decompress(const void* codes, int64_t code_pitch, const void* ex
  * Backward: g = grad * weight, grad_input = rstd * (g - xn * mean(g * xn)) + grad_sum, grad_weight = sum
  * over the rows of grad * xn.  grad_input is the gradient of x and of the residual alike; grad_sum (NULL:
  * none) is the gradient that arrives at h.  grad_input or grad_weight may be NULL.  `workspace`
- * (with grad_weight): DEVICE scratch of optimi_b200_rms_norm_backward_workspace_bytes(rows, cols) bytes,
+ * (with grad_weight; may be 0 bytes): DEVICE scratch of optimi_b200_rms_norm_backward_workspace_bytes(rows, cols, dtype) bytes,
  * 16-byte aligned.  Sums are taken in a fixed order. */
 int optimi_b200_rms_norm(const void* x, int64_t x_stride, const void* residual, int64_t residual_stride, const void* weight,
                          int64_t rows, int64_t cols, double eps, int dtype, void* y, void* sum, void* codes, int64_t code_pitch,
                          void* exponents, int64_t exponent_pitch, float* rstd, void* stream);
-size_t optimi_b200_rms_norm_backward_workspace_bytes(int64_t rows, int64_t cols);
+size_t optimi_b200_rms_norm_backward_workspace_bytes(int64_t rows, int64_t cols, int dtype);
 int optimi_b200_rms_norm_backward(const void* grad, int64_t grad_stride, const void* grad_sum, int64_t grad_sum_stride,
                                   const void* codes, int64_t code_pitch, const void* exponents, int64_t exponent_pitch,
                                   const float* rstd, const void* weight, int64_t rows, int64_t cols, int dtype, void* grad_input,

@@ -62,7 +62,7 @@ def _load() -> ctypes.CDLL:
         fn.argtypes = argtypes
         fn.restype = _I
     lib.optimi_b200_rms_norm_backward_workspace_bytes.restype = _Z
-    lib.optimi_b200_rms_norm_backward_workspace_bytes.argtypes = [_L, _L]
+    lib.optimi_b200_rms_norm_backward_workspace_bytes.argtypes = [_L, _L, _I]
     lib.optimi_b200_weight_gradient_workspace_bytes.restype = _Z
     lib.optimi_b200_weight_gradient_workspace_bytes.argtypes = [_L, _L, _L]
     lib.optimi_b200_last_error.restype = ctypes.c_char_p

@@ -304,12 +304,13 @@ class _RMSNorm(torch.autograd.Function):
         rows, cols = g.shape
         dx = _dense_like(grad) if need_x or need_r else None
         dw = torch.empty_like(w) if need_w else None
-        need = _lib.LIB.optimi_b200_rms_norm_backward_workspace_bytes(rows, cols) if need_w else 0
+        code = _lib.DTYPE_CODE[grad.dtype]
+        need = _lib.LIB.optimi_b200_rms_norm_backward_workspace_bytes(rows, cols, code) if need_w else 0
         workspace = torch.empty(need, dtype=torch.uint8, device=grad.device) if need else None
         at, groups = buffer.data_ptr(), -(-cols // GROUP)
         _call(_lib.LIB.optimi_b200_rms_norm_backward, grad.device, g.data_ptr(), g.stride(0), _ptr(s), 0 if s is None else s.stride(0),
               at, groups * GROUP, at + rows * groups * GROUP, groups, at + _buffer_bytes(rows, cols)[1], _ptr(w), rows, cols,
-              _lib.DTYPE_CODE[grad.dtype], _ptr(dx), _ptr(dw), _ptr(workspace), need)  # fmt: skip
+              code, _ptr(dx), _ptr(dw), _ptr(workspace), need)  # fmt: skip
         return dx if need_x else None, dw, dx if need_r else None, None, None
 
 

@@ -397,7 +397,8 @@ __global__ void long_rms_norm_kernel(const T* __restrict__ x, int64_t xs, const 
 // Backward, from the 8-bit xn:  g = dy * w    m = mean(g * xn)    dx = rstd * (g - xn * m) + dsum    dw = sum over rows of dy * xn
 //
 // A block keeps its threads' columns of dw in registers over all its rows, and leaves one line of partial sums in the workspace
-// (its row groups added up in order in shared memory); a second kernel adds up the lines in order.  Few blocks, so few lines.
+// (its row groups added up in order in shared memory); a second kernel adds up the lines in order.  Few blocks, so few lines; with
+// few rows one block takes them all and writes dw itself (`direct`): the second launch costs more than up to four rows in turn.
 // The next row is asked for before this one is reduced (kAhead), so that loads are always under way.  Long rows (K > 2) have no
 // registers for that, nor for the weight, which they read again for every row, nor for dsum, asked for after the first pass.
 template <typename T, int K, bool kAny>
@@ -412,7 +413,8 @@ template <typename T, int P, int K, bool kAny>
 __global__ void __launch_bounds__(512, 1)
     rms_norm_backward_kernel(const T* __restrict__ grad, int64_t gs, const T* __restrict__ grad_sum, int64_t hs, const int8_t* __restrict__ codes,
                              int64_t pitch, const uint8_t* __restrict__ exponents, int64_t epitch, const float* __restrict__ rstd,
-                             const T* __restrict__ weight, int64_t rows, int cols, T* __restrict__ dx, float* __restrict__ lines) {
+                             const T* __restrict__ weight, int64_t rows, int cols, T* __restrict__ dx, float* __restrict__ lines,
+                             T* __restrict__ direct) {
   using Values = Chunk<T>;
   constexpr bool kAhead = K <= 2;
   constexpr int C = Values::C, kThreads = 512, kGroups = kThreads / P;
@@ -508,14 +510,16 @@ __global__ void __launch_bounds__(512, 1)
     if constexpr (kAhead) v = next;
     else ask(row + step, v);
   }
-  if (!lines) return;
+  if (!lines && !direct) return;
   if constexpr (kGroups == 1) {
 #pragma unroll
     for (int k = 0; k < K; k++)
 #pragma unroll
       for (int i = 0; i < C; i++) {
         const int c = (k * P + t) * C + i;
-        if (c < cols) lines[(int64_t)blockIdx.x * cols + c] = dw[k][i];
+        if (c >= cols) continue;
+        if (direct) direct[c] = from_f32<T>(dw[k][i]);
+        else lines[(int64_t)blockIdx.x * cols + c] = dw[k][i];
       }
   } else {
 #pragma unroll
@@ -527,7 +531,8 @@ __global__ void __launch_bounds__(512, 1)
       float s = sums[0][c];
 #pragma unroll
       for (int j = 1; j < kGroups; j++) s += sums[j][c];
-      lines[(int64_t)blockIdx.x * cols + c] = s;
+      if (direct) direct[c] = from_f32<T>(s);
+      else lines[(int64_t)blockIdx.x * cols + c] = s;
     }
   }
 }
@@ -774,12 +779,18 @@ int optimi_b200_rms_norm(const void* x, int64_t x_stride, const void* residual, 
   return launched(fn);
 }
 
-// Blocks of the backward pass, and so lines of its workspace: the kernels for rows in registers take at most 148 blocks, the one
-// for long rows four times as many.
+// Whether one block takes all rows of the backward pass.
+static bool one_block(int64_t rows, int64_t cols, int size) {
+  const Deal d = deal_of(cols, size, kBackwardAnyChunks);
+  return d.K > 0 && rows <= 4 * (512 / d.P);
+}
+
+// Lines of the backward pass's workspace: the kernels for rows in registers take at most 148 blocks, the one for long rows four times
+// as many.
 static unsigned backward_blocks(int64_t rows) { return grid_of(rows, kLongBlocks); }
 
-size_t optimi_b200_rms_norm_backward_workspace_bytes(int64_t rows, int64_t cols) {
-  if (rows <= 0 || cols <= 0) return 0;
+size_t optimi_b200_rms_norm_backward_workspace_bytes(int64_t rows, int64_t cols, int dtype) {
+  if (rows <= 0 || cols <= 0 || !known_dtype(dtype) || one_block(rows, cols, dtype == OPTIMI_F32 ? 4 : 2)) return 0;
   return (size_t)backward_blocks(rows) * (size_t)cols * sizeof(float);
 }
 
@@ -800,14 +811,15 @@ int optimi_b200_rms_norm_backward(const void* grad, int64_t grad_stride, const v
   if (!grad_input && !grad_weight) return OPTIMI_OK;
   rc = check_codes(fn, codes, code_pitch, exponents, exponent_pitch, cols);
   if (rc != OPTIMI_OK) return rc;
-  const size_t need = optimi_b200_rms_norm_backward_workspace_bytes(rows, cols);
-  if (grad_weight && (!workspace || workspace_bytes < need))
+  const size_t need = optimi_b200_rms_norm_backward_workspace_bytes(rows, cols, dtype);
+  if (grad_weight && need > 0 && (!workspace || workspace_bytes < need))
     return fail(OPTIMI_ERR_WORKSPACE_TOO_SMALL, "%s: workspace has %zu bytes, %zu are needed", fn, workspace ? workspace_bytes : (size_t)0, need);
   const int size = dtype == OPTIMI_F32 ? 4 : 2;
   const bool any = cols * size % 16 || !rows_aligned(grad, grad_stride, rows, size) || (grad_sum && !rows_aligned(grad_sum, grad_sum_stride, rows, size)) ||
                    !aligned(weight, 16) || !aligned(grad_input, 16);
   const Deal d = deal_of(cols, size, any ? kBackwardAnyChunks : kBackwardChunks);
-  float* lines = grad_weight ? (float*)workspace : nullptr;
+  const bool alone = one_block(rows, cols, size);
+  float* lines = grad_weight && !alone ? (float*)workspace : nullptr;
   unsigned blocks = 0;
   FOR_DTYPE(dtype, {
     if (d.K == 0) {
@@ -819,17 +831,17 @@ int optimi_b200_rms_norm_backward(const void* grad, int64_t grad_stride, const v
       const auto with_constants = [&](auto p, auto k, auto is_any) {
         constexpr int P = decltype(p)::value, K = decltype(k)::value;
         constexpr bool kIsAny = decltype(is_any)::value;
-        blocks = grid_of((rows + 512 / P - 1) / (512 / P), kBackwardBlocks);
+        blocks = alone ? 1 : grid_of((rows + 512 / P - 1) / (512 / P), kBackwardBlocks);
         rms_norm_backward_kernel<T, P, K, kIsAny><<<blocks, 512, 0, s>>>(
             (const T*)grad, grad_stride, (const T*)grad_sum, grad_sum_stride, (const int8_t*)codes, code_pitch, (const uint8_t*)exponents,
-            exponent_pitch, rstd, (const T*)weight, rows, (int)cols, (T*)grad_input, lines);
+            exponent_pitch, rstd, (const T*)weight, rows, (int)cols, (T*)grad_input, lines, alone ? (T*)grad_weight : nullptr);
       };
       if (any) with_deal<T, kBackwardAnyChunks>(d, [&](auto p, auto k) { with_constants(p, k, std::true_type()); });
       else with_deal<T, kBackwardChunks>(d, [&](auto p, auto k) { with_constants(p, k, std::false_type()); });
     }
   });
   rc = launched(fn);
-  if (rc != OPTIMI_OK || !grad_weight) return rc;
+  if (rc != OPTIMI_OK || !lines) return rc;
   FOR_DTYPE(dtype, (line_sum_kernel<T><<<(unsigned)((cols + 31) / 32), 512, 0, s>>>(lines, (int)blocks, cols, (T*)grad_weight)));
   return launched(fn);
 }

@@ -86,7 +86,7 @@ def test_entry_points_reject_bad_arguments_without_launching():
     refused(L.optimi_b200_rms_norm(*with_(norm, _7=float("nan"))), b"eps")
     refused(L.optimi_b200_rms_norm(*with_(norm, _11=p, _12=64, _13=p, _14=2)), b"go together")
     refused(L.optimi_b200_rms_norm(*with_(norm, _15=p)), b"codes or exponents is NULL")
-    back = [p, 64, None, 0, p, 64, p, 2, p, None, 4, 64, 1, p, p, p, 1 << 20, None]
+    back = [p, 64, None, 0, p, 64, p, 2, p, None, 400, 64, 1, p, p, p, 1 << 20, None]
     refused(L.optimi_b200_rms_norm_backward(*with_(back, _0=None)), b"grad or rstd is NULL")
     refused(L.optimi_b200_rms_norm_backward(*with_(back, _8=None)), b"grad or rstd is NULL")
     refused(L.optimi_b200_rms_norm_backward(*with_(back, _16=8)), b"workspace", -3)
@@ -152,5 +152,7 @@ def test_preparing_a_model_changes_only_what_it_says():
 
 def test_workspaces_grow_with_the_problem():
     L = _lib.LIB
-    assert L.optimi_b200_rms_norm_backward_workspace_bytes(0, 64) == 0
-    assert 0 < L.optimi_b200_rms_norm_backward_workspace_bytes(1, 64) < L.optimi_b200_rms_norm_backward_workspace_bytes(1000, 64)
+    assert L.optimi_b200_rms_norm_backward_workspace_bytes(0, 64, 1) == 0
+    assert L.optimi_b200_rms_norm_backward_workspace_bytes(1, 64, 1) == 0  # one block adds up the rows itself
+    assert 0 < L.optimi_b200_rms_norm_backward_workspace_bytes(100, 64, 1) < L.optimi_b200_rms_norm_backward_workspace_bytes(1000, 64, 1)
+    assert L.optimi_b200_rms_norm_backward_workspace_bytes(1000, 64, 9) == 0
