@@ -345,10 +345,12 @@ struct CodeChunk {
     if constexpr (C == 8) *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
     else *reinterpret_cast<uint32_t*>(p) = w[0];
   }
+  // Code i times a unit of at most 2^100, given the unit and scaled_offset(unit): exact, so one fused operation does for both.
+  static __device__ __forceinline__ float scaled_offset(float unit) { return __fmul_rn(-8388736.0f, unit); }
+  __device__ __forceinline__ float get_scaled(int i, float unit, float offset) const { return __fmaf_rn(raw(i), unit, offset); }
   // Code i as fp32: the byte with its sign bit flipped, set into the low bits of 2^23, is 2^23 + 128 + code.
-  __device__ __forceinline__ float get(int i) const {
-    return __uint_as_float(__byte_perm(w[i / 4] ^ 0x80808080u, 0x4b000000u, 0x7440 + i % 4)) - 8388736.0f;
-  }
+  __device__ __forceinline__ float raw(int i) const { return __uint_as_float(__byte_perm(w[i / 4] ^ 0x80808080u, 0x4b000000u, 0x7440 + i % 4)); }
+  __device__ __forceinline__ float get(int i) const { return raw(i) - 8388736.0f; }
 };
 
 // 2^(e - 127) for two exponent bytes, as a pair of T.  bf16: the byte is the exponent field (255 gives an infinity, which

@@ -470,13 +470,14 @@ __global__ void __launch_bounds__(512, 1)
     for (int k = 0; k < K; k++) {
       const int c = (k * P + t) * C;
       g[k] = v.g[k].settle(grad + row * gs + c, cols - c);
-      const float unit = power_of((int)v.e[k]);
+      // |xn| is below sqrt(cols), so a unit is far below 2^100 (or infinite, of a NaN group, which stays NaN)
+      const float unit = power_of((int)v.e[k]), offset = v.code[k].scaled_offset(unit);
       Values wk;
       if constexpr (kAhead) wk = w[k];
       else wk = weights(k);
 #pragma unroll
       for (int i = 0; i < C; i++) {
-        const float n = __fmul_rn(v.code[k].get(i), unit), d = g[k].get(i);
+        const float n = v.code[k].get_scaled(i, unit, offset), d = g[k].get(i);
         dw[k][i] = __fmaf_rn(d, n, dw[k][i]);
         m = __fmaf_rn(weight ? __fmul_rn(d, wk.get(i)) : d, n, m);
       }
@@ -484,23 +485,21 @@ __global__ void __launch_bounds__(512, 1)
     if (dx) {
       if constexpr (!kAhead) ask_sum(row, v);
       m = row_sum<P, float>(m, part[group], turn, group) / (float)cols;
+      const float mr = -__fmul_rn(m, v.r);
 #pragma unroll
       for (int k = 0; k < K; k++) {
         const int c = (k * P + t) * C;
-        const float unit = power_of((int)v.e[k]);
-        Values wk;
+        const float unit = power_of((int)v.e[k]), offset = v.code[k].scaled_offset(unit);
+        Values wk, s;
         if constexpr (kAhead) wk = w[k];
         else wk = weights(k);
+        if (grad_sum) s = v.s[k].settle(grad_sum + row * hs + c, cols - c);
         float f[C];
 #pragma unroll
-        for (int i = 0; i < C; i++) {
-          const float n = __fmul_rn(v.code[k].get(i), unit), d = g[k].get(i);
-          f[i] = __fmul_rn(v.r, __fmaf_rn(-n, m, weight ? __fmul_rn(d, wk.get(i)) : d));
-        }
-        if (grad_sum) {
-          const Values s = v.s[k].settle(grad_sum + row * hs + c, cols - c);
-#pragma unroll
-          for (int i = 0; i < C; i++) f[i] = __fadd_rn(f[i], s.get(i));
+        for (int i = 0; i < C; i++) {  // rstd * g + dsum, then - xn * (m * rstd)
+          const float d = weight ? __fmul_rn(g[k].get(i), wk.get(i)) : g[k].get(i);
+          f[i] = grad_sum ? __fmaf_rn(v.r, d, s.get(i)) : __fmul_rn(v.r, d);
+          f[i] = __fmaf_rn(v.code[k].get_scaled(i, unit, offset), mr, f[i]);
         }
         Values out;
         out.set(f);
