@@ -7,6 +7,11 @@
 // instruction may lie there: a row per channel, tokens along the columns.  That costs shared memory only the codes' own
 // bytes (one read of 8 bits a value) where a 16-bit copy beside dY would be written and then read again.
 // code * 2^k has 7 bits and fits bf16 and fp16 exactly, so the products are those of the restored activation.
+//
+// What bounds it: the tensor cores and the card's power.  8192 tokens, 14336 outputs x 4096 channels, bf16: 615 us alone
+// (1564 TFLOP/s, 0.94 of the measured product rate) and 735 to 755 us in a long run, where the clock falls to 1.3 GHz (a 16-bit
+// product of the same sizes by the vendor's library: 618 and 716 us there).  4096 x 1024: 58 us, 64 tiles on 74 pairs, the
+// tensor cores of those 94 % busy.  With few tokens it is the results' way to memory (64 tokens, 4096 x 4096: 23 us).
 #include "activation_common.cuh"
 
 #include <cuda.h>
@@ -16,8 +21,10 @@ namespace act {
 
 // A pair of blocks on two neighbouring SMs works on one tile of 256 channels x 384 outputs (or 256), 64 tokens at a time.  Each
 // holds the codes, X^T and the results of its 128 channels, and the gradients of half of the outputs; the instruction reads
-// the other half from the partner's shared memory.  A tile is that wide because the conversion of codes, done once a tile and
-// step, is what the multiplications wait for (measured at 256 outputs: 0.41 us a step, of which 0.32 us without conversion).
+// the other half from the partner's shared memory (one block with 128 x 256 of its own loaded twice the gradients: 1175 us for the
+// call above, where the pair at first took 768).  A tile is that wide because the conversion of codes, done once a tile and step,
+// competes with the multiplications for issue slots and power: 384 outputs 615 us, 256 outputs 670 us.  Seven stages, eight slots or
+// a third set of converting warps gained nothing.
 constexpr int kM = 128, kN = 384, kK = 64;           // channels of a block, most outputs of the pair, tokens of a step
 constexpr int kNarrow = 256;                         // outputs of the first instruction; the second takes the others
 constexpr int kStages = 6;                           // of gradients and codes, in shared memory
@@ -111,7 +118,8 @@ static __device__ __forceinline__ void multiply(uint32_t d, uint32_t a, uint64_t
                : "memory");
 }
 
-// What the pairs of blocks do.  `whole` tiles are dealt out in turns, all their tokens at once, so that the pairs of one turn
+// What the pairs of blocks do.  (A block per tile, started anew for each, lost 9 us a tile to its start and to storing results: the
+// pairs stay, and results are stored while the next tile is multiplied.)  `whole` tiles are dealt out in turns, all their tokens at once, so that the pairs of one turn
 // read the same tokens at the same time (from L2); the tiles that would not fill another turn are cut into `slices` along
 // the tokens, whose sums go to the workspace in fp32 and are added up in order by a second kernel.
 struct Plan {
@@ -461,8 +469,10 @@ __global__ void __launch_bounds__(256) join_slices_kernel(const float4* __restri
   }
 }
 
-// What a call costs, in steps of a tile of 256 outputs (0.38 us): a step of 384 outputs is kWideStep of them; slices cost a launch and,
-// each, a trip of its sums through L2.  Of the two widths the cheaper is taken, and slices only where they are cheaper.
+// What a call costs, in steps of a tile of 256 outputs (0.38 us): a step of 384 outputs is kWideStep of them (0.47 to 0.58 us); slices
+// cost a launch and, each, a trip of its sums through L2.  Of the two widths the cheaper is taken, and slices only where they are
+// cheaper.  8192 tokens: 14336 x 4096 615 us wide, 666 narrow; 4096 x 1024 74 wide, 58 narrow; 16384 tokens, 256 x 256: 20 us in
+// 74 slices, about 100 in one.
 constexpr float kWideStep = 1.4f, kJoin = 10.0f, kPiece = 0.1f;
 
 static Plan plan_of_width(int64_t rows, int64_t outputs, int64_t channels, int pairs, int width, float* cost) {
@@ -535,15 +545,22 @@ static int make_map(const char* fn, CUtensorMap* map, CUtensorMapDataType type, 
 }
 
 template <typename T>
-static int launch_weight_gradient(const char* fn, const CUtensorMap& grad_map, const CUtensorMap& code_map, const void* exponents,
+static int launch_weight_gradient(const char* fn, const void* grad, int64_t grad_stride, const void* codes, int64_t pitch, const void* exponents,
                                   int64_t epitch, const void* channel_scale, const Plan& plan, int pairs, void* dw, void* workspace,
                                   cudaStream_t s) {
+  // First a call of the runtime: it makes the device's context current, which a thread without any CUDA call so far (autograd's,
+  // for one) lacks, and which the driver's encoder of tensor maps asks for.
   cudaError_t e = cudaFuncSetAttribute(weight_gradient_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes);
   if (e != cudaSuccess) return fail(OPTIMI_ERR_CUDA, "%s: %s", fn, cudaGetErrorString(e));
+  CUtensorMap grad_map, code_map;
+  constexpr CUtensorMapDataType kType = std::is_same<T, __half>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+  int rc = make_map(fn, &grad_map, kType, grad, plan.outputs, plan.rows, grad_stride * 2, 64, kK);
+  if (rc == OPTIMI_OK) rc = make_map(fn, &code_map, CU_TENSOR_MAP_DATA_TYPE_UINT8, codes, plan.channels, plan.rows, pitch, kM, kK);
+  if (rc != OPTIMI_OK) return rc;
   const int64_t items = (int64_t)plan.whole + (int64_t)plan.cut * plan.slices;
   weight_gradient_kernel<T><<<(unsigned)(2 * (items < pairs ? items : pairs)), kThreads, kSmemBytes, s>>>(
       grad_map, code_map, (const uint8_t*)exponents, epitch, (const T*)channel_scale, plan, (T*)dw, (float*)workspace);
-  int rc = launched(fn);
+  rc = launched(fn);
   if (rc != OPTIMI_OK || plan.cut == 0) return rc;
   if (plan.slices > 8)
     join_slices_kernel<T, true><<<dim3(plan.width, 2, plan.cut), 256, 0, s>>>((const float4*)workspace, plan, (const T*)channel_scale, (T*)dw);
@@ -603,16 +620,11 @@ int optimi_b200_weight_gradient(const void* grad, int64_t grad_stride, const voi
   if (need > 0 && (!workspace || workspace_bytes < need || !aligned(workspace, 16)))
     return fail(OPTIMI_ERR_WORKSPACE_TOO_SMALL, "%s: workspace has %zu bytes, %zu are needed, 16-byte aligned", fn,
                 workspace ? workspace_bytes : (size_t)0, need);
-  CUtensorMap grad_map, code_map;
-  rc = make_map(fn, &grad_map, dtype == OPTIMI_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, grad, outputs, rows,
-                grad_stride * 2, 64, kK);
-  if (rc != OPTIMI_OK) return rc;
-  rc = make_map(fn, &code_map, CU_TENSOR_MAP_DATA_TYPE_UINT8, codes, channels, rows, code_pitch, kM, kK);
-  if (rc != OPTIMI_OK) return rc;
   if (dtype == OPTIMI_BF16)
-    return launch_weight_gradient<__nv_bfloat16>(fn, grad_map, code_map, exponents, exponent_pitch, channel_scale, plan, pairs, grad_weight,
-                                                 workspace, s);
-  return launch_weight_gradient<__half>(fn, grad_map, code_map, exponents, exponent_pitch, channel_scale, plan, pairs, grad_weight, workspace, s);
+    return launch_weight_gradient<__nv_bfloat16>(fn, grad, grad_stride, codes, code_pitch, exponents, exponent_pitch, channel_scale, plan, pairs,
+                                                 grad_weight, workspace, s);
+  return launch_weight_gradient<__half>(fn, grad, grad_stride, codes, code_pitch, exponents, exponent_pitch, channel_scale, plan, pairs,
+                                        grad_weight, workspace, s);
 }
 
 }  // extern "C"

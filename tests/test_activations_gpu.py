@@ -758,6 +758,32 @@ def test_lazily_negated_views():
     assert torch.equal(got.codes, want.codes) and torch.equal(got.exponents, want.exponents)
 
 
+def test_first_call_of_a_thread():
+    """A thread that made no CUDA call yet (as autograd's own, when the input needs no gradient) has no current context."""
+    import threading
+
+    a = act()
+    x, dy = loud((96, 128), torch.bfloat16, 1).cuda(), normal((96, 64), torch.bfloat16, 2).cuda()
+    saved = a.compress(x)
+    want = a.weight_gradient(dy, saved)
+    torch.empty_like(want), torch.empty_like(want)
+    torch.cuda.synchronize()
+    got = []
+
+    def work():
+        try:
+            got.append(a.weight_gradient(dy, saved))
+        except RuntimeError as e:
+            got.append(e)
+
+    t = threading.Thread(target=work)
+    t.start()
+    t.join()
+    torch.cuda.synchronize()
+    assert isinstance(got[0], torch.Tensor), got[0]
+    assert same_bits(got[0], want)
+
+
 def test_calls_from_two_threads():
     import threading
 
