@@ -8,6 +8,7 @@ own message.
 from __future__ import annotations
 
 import ctypes
+import importlib.util
 
 import torch
 
@@ -109,8 +110,17 @@ def _load() -> ctypes.CDLL:
     return lib
 
 
+def _load_host():
+    """The C++ module beside the library (optimi_b200/csrc/activations_host.cpp); it links against the library loaded above."""
+    spec = importlib.util.spec_from_file_location("_host", _build.HOST_LIB)
+    module = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(module)
+    return module
+
+
 LIB = _load()
 LIB_PATH = _build.LIB
+HOST = _load_host()
 
 
 class peer_push:

@@ -25,7 +25,6 @@ from typing import Any, NamedTuple
 from warnings import warn
 
 import torch
-import torch.nn.functional as F
 import torch.utils.checkpoint
 from torch import Tensor, nn
 
@@ -79,24 +78,15 @@ class CompressedActivation:
 
     @classmethod
     def _of(cls, tensors: Sequence[Tensor], shape, dtype, channel_scale=None) -> CompressedActivation:
-        """From what `_tensors` gave, or one buffer of `_buffer_bytes` that holds the codes, then the exponents; no checks."""
+        """From what `_tensors` gives: two tensors, or one buffer that holds the codes, then the exponents; no checks."""
         self = object.__new__(cls)
         self._codes, self._exponents, self._buffer = (*tensors, None) if len(tensors) == 2 else (None, None, tensors[0])
         self.shape, self.dtype, self.channel_scale = shape, dtype, channel_scale
         return self
 
     def _tensors(self) -> tuple[Tensor, ...]:
-        """What holds the codes and exponents, to be kept with `ctx.save_for_backward`."""
+        """What holds the codes and exponents."""
         return (self._codes, self._exponents) if self._buffer is None else (self._buffer,)
-
-    def _layout(self) -> tuple[int, int, int, int]:
-        """Addresses and pitches of codes and exponents."""
-        if self._buffer is None:
-            c, e = self._codes, self._exponents
-            return c.data_ptr(), c.stride(0), e.data_ptr(), e.stride(0)
-        rows, groups = _rows(self.shape), -(-self.shape[-1] // GROUP)
-        at = self._buffer.data_ptr()
-        return at, groups * GROUP, at + rows * groups * GROUP, groups
 
     @property
     def codes(self) -> Tensor:
@@ -138,7 +128,7 @@ class RMSNormOutput(NamedTuple):
 
 
 # ---------------------------------------------------------------------------------------------
-# calls of the kernels
+# operators: checks of arguments, autograd nodes and kernel calls are in csrc/activations_host.cpp
 # ---------------------------------------------------------------------------------------------
 
 
@@ -149,175 +139,23 @@ def _rows(shape) -> int:
     return rows
 
 
-def _check(name: str, what: str, t: Tensor, like: Tensor | None = None) -> None:
-    if not t.is_cuda:
-        raise RuntimeError(f"{name}: `{what}` lives on {t.device}; optimi_b200 takes CUDA tensors only (there is no CPU path)")
-    if t.dtype not in _lib.DTYPE_CODE:
-        raise RuntimeError(f"{name}: `{what}` has unsupported dtype {t.dtype} (float32, bfloat16 and float16 are)")
-    if like is not None and (t.device != like.device or t.dtype != like.dtype):
-        raise RuntimeError(f"{name}: `{what}` ({t.dtype}, {t.device}) does not match {like.dtype} on {like.device}")
-
-
-def _as_rows(t: Tensor) -> Tensor:
-    """`t` as a matrix of its last dimension whose rows are contiguous and do not overlap: itself where that holds, else a copy."""
-    if t.is_neg():  # a lazily negated view: its memory holds the opposite
-        t = t.detach().resolve_neg()
-    if t.dim() != 2:
-        t = t.detach().reshape(_rows(t.shape), t.shape[-1])
-    if t.is_contiguous():
-        return t
-    if t.shape[1] != 1 and t.stride(1) != 1 or t.shape[0] > 1 and t.stride(0) < t.shape[1]:
-        t = t.detach().contiguous()
-    return t
-
-
-def _ptr(t: Tensor | None) -> int | None:
-    return None if t is None else t.data_ptr()
-
-
-def _stream(device: torch.device) -> int:
-    # torch.cuda.current_stream(device).cuda_stream without the Stream object around it (2 us of a 15 us call)
-    return torch._C._cuda_getCurrentRawStream(device.index)
-
-
-def _call(fn, device: torch.device, *args) -> None:
-    """Calls entry point `fn` with `args` and the current stream of `device`, that device being current."""
-    if torch.cuda.current_device() == device.index:
-        rc = fn(*args, _stream(device))
-    else:
-        with torch.cuda.device(device):
-            rc = fn(*args, _stream(device))
-    if rc:
-        _lib.check(rc)
-
-
-def _dense_like(t: Tensor) -> Tensor:
-    """A new contiguous tensor of `t`'s shape and type."""
-    return torch.empty_like(t) if t.is_contiguous() else torch.empty(t.shape, dtype=t.dtype, device=t.device)
-
-
-def _buffer_bytes(rows: int, cols: int) -> tuple[int, int]:
-    """Bytes of codes and exponents in one buffer, and where 4-byte values may follow them."""
-    n = rows * -(-cols // GROUP) * (GROUP + 1)
-    return n, -(-n // 16) * 16
-
-
 def compress(x: Tensor) -> CompressedActivation:
     """`x` (float32, bfloat16 or float16; any shape with at least one dimension) in 8 bits.  Takes no part in autograd."""
-    _check("compress", "x", x)
-    if x.dim() == 0:
-        raise RuntimeError("compress: `x` must have at least one dimension")
-    m = _as_rows(x)
-    rows, cols = m.shape
-    device = x.device
-    saved = CompressedActivation._of((torch.empty(_buffer_bytes(rows, cols)[0], dtype=torch.uint8, device=device),), x.shape, x.dtype)
-    _call(_lib.LIB.optimi_b200_compress, device, m.data_ptr(), m.stride(0), rows, cols, _lib.DTYPE_CODE[x.dtype], *saved._layout())
-    return saved
+    return CompressedActivation._of((_lib.HOST.compress(x),), x.shape, x.dtype)
 
 
 def decompress(saved: CompressedActivation) -> Tensor:
     """The activation `saved` stands for, its `channel_scale` applied."""
-    device = saved.device
-    if device.type != "cuda":
-        raise RuntimeError(f"decompress: `saved` lives on {device}; optimi_b200 takes CUDA tensors only (there is no CPU path)")
-    out = torch.empty(saved.shape, dtype=saved.dtype, device=device)
-    scale = None if saved.channel_scale is None else saved.channel_scale.detach().contiguous()
-    _call(_lib.LIB.optimi_b200_decompress, device, *saved._layout(), _ptr(scale), _rows(saved.shape), saved.shape[-1],
-          _lib.DTYPE_CODE[saved.dtype], out.data_ptr())  # fmt: skip
-    return out
+    return _lib.HOST.decompress(saved._tensors(), saved.shape, saved.dtype, saved.channel_scale)
 
 
 def weight_gradient(grad: Tensor, saved: CompressedActivation) -> Tensor:
     """Gradient of a linear layer's weight, ``grad^T @ saved`` summed over all tokens: (outputs, channels), in `grad`'s type.
 
     `grad` (bfloat16 or float16) has the leading dimensions of `saved.shape`.  The kept activation goes to the tensor
-    cores as it is (its values are exact in 16 bits); sums are held in 32 bits.
+    cores as it is (its values are exact in 16 bits); sums are held in 32 bits.  Takes no part in autograd.
     """
-    name = "weight_gradient"
-    _check(name, "grad", grad)
-    if grad.dtype == torch.float32:
-        raise RuntimeError(f"{name}: `grad` is float32; bfloat16 and float16 are supported")
-    if saved.dtype != grad.dtype or saved.device != grad.device:
-        raise RuntimeError(f"{name}: `saved` ({saved.dtype}, {saved.device}) does not match `grad` ({grad.dtype}, {grad.device})")
-    if grad.dim() == 0 or _rows(grad.shape) != _rows(saved.shape):
-        raise RuntimeError(f"{name}: `grad` {tuple(grad.shape)} and `saved` {tuple(saved.shape)} have different numbers of tokens")
-    m = _as_rows(grad.detach())
-    rows, outputs = m.shape
-    channels = saved.shape[-1]
-    device, code = grad.device, _lib.DTYPE_CODE[grad.dtype]
-    pitch = -(-outputs // 8) * 8
-    copied = m.data_ptr() % 16 != 0 or (m.stride(0) if rows > 1 else outputs) % 8 != 0  # the kernel loads rows that begin on 16 bytes
-    stride = pitch if copied or rows <= 1 else m.stride(0)
-    dw = torch.empty((outputs, channels), dtype=grad.dtype, device=device)
-    scale = None if saved.channel_scale is None else saved.channel_scale.detach().contiguous()
-    need = _lib.LIB.optimi_b200_weight_gradient_workspace_bytes(rows, outputs, channels)
-    workspace = torch.empty(need, dtype=torch.uint8, device=device) if need else None
-    if copied:
-        source, m = m, torch.empty((rows, pitch), dtype=grad.dtype, device=device)
-        _call(_lib.LIB.optimi_b200_align_rows, device, source.data_ptr(), source.stride(0), rows, outputs, code, m.data_ptr(), pitch)
-    _call(_lib.LIB.optimi_b200_weight_gradient, device, m.data_ptr(), stride, *saved._layout(), _ptr(scale), rows, outputs, channels,
-          code, dw.data_ptr(), _ptr(workspace), need)  # fmt: skip
-    return dw
-
-
-def _norm_forward(x: Tensor, weight: Tensor | None, residual: Tensor | None, eps: float, keep: bool):
-    """(output, sum, buffer): the buffer holds the 8-bit form of the normalised rows and, behind it, their 1 / rms."""
-    m = _as_rows(x)
-    r = None if residual is None else _as_rows(residual)
-    rows, cols = m.shape
-    device = x.device
-    y = _dense_like(x)
-    h = None if r is None else _dense_like(x)
-    buffer = None
-    kept = (None, 0, None, 0, None)
-    if keep:
-        _, after = _buffer_bytes(rows, cols)
-        buffer = torch.empty(after + 4 * rows, dtype=torch.uint8, device=device)
-        at, groups = buffer.data_ptr(), -(-cols // GROUP)
-        kept = (at, groups * GROUP, at + rows * groups * GROUP, groups, at + after)
-    _call(_lib.LIB.optimi_b200_rms_norm, device, m.data_ptr(), m.stride(0), _ptr(r), 0 if r is None else r.stride(0), _ptr(weight),
-          rows, cols, eps, _lib.DTYPE_CODE[x.dtype], y.data_ptr(), _ptr(h), *kept)  # fmt: skip
-    return y, h, buffer
-
-
-class _RMSNorm(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, weight, residual, eps, kept):
-        w = None if weight is None else weight.contiguous()
-        y, h, buffer = _norm_forward(x, w, residual, eps, True)
-        kept.append(buffer)
-        ctx.save_for_backward(buffer, weight)
-        ctx.set_materialize_grads(False)
-        return y, h
-
-    @staticmethod
-    def backward(ctx, grad, grad_sum):
-        _refuse_double_backward("rms_norm")
-        buffer, weight = ctx.saved_tensors
-        need_x, need_w, need_r = ctx.needs_input_grad[:3]
-        if grad is None:  # only the residual was used: it passes through
-            dw = torch.zeros_like(weight) if need_w else None
-            return grad_sum if need_x else None, dw, grad_sum if need_r else None, None, None
-        g = _as_rows(grad)
-        s = None if grad_sum is None else _as_rows(grad_sum)
-        w = None if weight is None else weight.contiguous()
-        rows, cols = g.shape
-        dx = _dense_like(grad) if need_x or need_r else None
-        dw = torch.empty_like(w) if need_w else None
-        code = _lib.DTYPE_CODE[grad.dtype]
-        need = _lib.LIB.optimi_b200_rms_norm_backward_workspace_bytes(rows, cols, code) if need_w else 0
-        workspace = torch.empty(need, dtype=torch.uint8, device=grad.device) if need else None
-        at, groups = buffer.data_ptr(), -(-cols // GROUP)
-        _call(_lib.LIB.optimi_b200_rms_norm_backward, grad.device, g.data_ptr(), g.stride(0), _ptr(s), 0 if s is None else s.stride(0),
-              at, groups * GROUP, at + rows * groups * GROUP, groups, at + _buffer_bytes(rows, cols)[1], _ptr(w), rows, cols,
-              code, _ptr(dx), _ptr(dw), _ptr(workspace), need)  # fmt: skip
-        return dx if need_x else None, dw, dx if need_r else None, None, None
-
-
-def _refuse_double_backward(name: str) -> None:
-    # gradients are recorded inside a backward pass only under create_graph=True, and these kernels' would come out as constants
-    if torch.is_grad_enabled():
-        raise RuntimeError(f"{name}: differentiating the backward pass (create_graph=True) is not supported")
+    return _lib.HOST.weight_gradient(grad, saved._tensors(), saved.shape, saved.dtype, saved.channel_scale)
 
 
 def rms_norm(x: Tensor, weight: Tensor | None = None, residual: Tensor | None = None, *, eps: float | None = None,
@@ -328,92 +166,23 @@ def rms_norm(x: Tensor, weight: Tensor | None = None, residual: Tensor | None = 
     the type's machine epsilon, as in `torch.nn.RMSNorm`.  Where gradients are wanted the normalised row is kept in 8 bits:
     the backward pass reads it, and `linear` can share it (`saved`).  `compress=True` keeps it without gradients too.
     """
-    name = "rms_norm"
-    _check(name, "x", x)
-    if x.dim() == 0:
-        raise RuntimeError(f"{name}: `x` must have at least one dimension")
-    if weight is not None:
-        _check(name, "weight", weight, x)
-        if weight.shape != x.shape[-1:]:
-            raise RuntimeError(f"{name}: `weight` {tuple(weight.shape)} does not match the last dimension of `x` {tuple(x.shape)}")
-    if residual is not None:
-        _check(name, "residual", residual, x)
-        if residual.shape != x.shape:
-            raise RuntimeError(f"{name}: `residual` {tuple(residual.shape)} does not match `x` {tuple(x.shape)}")
-    eps = torch.finfo(x.dtype).eps if eps is None else float(eps)
-    if not eps >= 0:
-        raise ValueError(f"{name}: eps={eps} must not be negative")
-    wants_grad = torch.is_grad_enabled() and (
-        x.requires_grad or (weight is not None and weight.requires_grad) or (residual is not None and residual.requires_grad)
-    )
-    if wants_grad:
-        kept: list[Tensor] = []
-        y, h = _RMSNorm.apply(x, weight, residual, eps, kept)
-        buffer = kept[0]
-    else:
-        w = None if weight is None else weight.detach().contiguous()
-        y, h, buffer = _norm_forward(x, w, residual, eps, compress)
-    saved = None if buffer is None else CompressedActivation._of((buffer,), x.shape, x.dtype, None if weight is None else weight.detach())
-    return RMSNormOutput(y, h, saved)
-
-
-class _Linear(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, weight, bias, saved):
-        out = F.linear(x, weight, bias)
-        ctx.shape = x.shape
-        ctx.keeps_weight = ctx.needs_input_grad[0]
-        keep = [weight] if ctx.keeps_weight else []
-        if ctx.needs_input_grad[1]:
-            if saved is None:
-                saved = compress(x)
-            keep += [saved.channel_scale, *saved._tensors()]
-        ctx.save_for_backward(*keep)
-        return out
-
-    @staticmethod
-    def backward(ctx, grad):
-        _refuse_double_backward("linear")
-        kept = list(ctx.saved_tensors)
-        dx = dw = db = None
-        if ctx.keeps_weight:
-            dx = grad @ kept.pop(0)
-        if ctx.needs_input_grad[1]:
-            scale, *tensors = kept
-            dw = weight_gradient(grad, CompressedActivation._of(tensors, ctx.shape, grad.dtype, scale))
-        if ctx.needs_input_grad[2]:
-            db = grad.reshape(-1, grad.shape[-1]).sum(0)
-        return dx, dw, db, None
+    output, new_residual, buffer = _lib.HOST.rms_norm(x, weight, residual, eps, compress)
+    if buffer is None:
+        return RMSNormOutput(output, new_residual, None)
+    saved = CompressedActivation._of((buffer,), x.shape, x.dtype, None if weight is None else weight.detach())
+    return RMSNormOutput(output, new_residual, saved)
 
 
 def linear(x: Tensor, weight: Tensor, bias: Tensor | None = None, *, saved: CompressedActivation | None = None) -> Tensor:
     """`torch.nn.functional.linear` that keeps its input in 8 bits for the weight gradient instead of `x` itself.
 
     `saved`: the 8-bit form of `x` where there is one already (`rms_norm`'s, or one `compress(x)` shared by several
-    layers); else `x` is compressed here, once the weight needs a gradient.  bfloat16 and float16; under autocast
+    layers); else `x` is compressed here, where the weight needs a gradient.  bfloat16 and float16; under autocast
     the arguments are cast as `torch.nn.functional.linear` casts them.
     """
-    name = "linear"
-    if torch.is_autocast_enabled("cuda") and x.is_cuda:
-        dtype = torch.get_autocast_dtype("cuda")
-        x, weight, bias = x.to(dtype), weight.to(dtype), None if bias is None else bias.to(dtype)
-    _check(name, "x", x)
-    _check(name, "weight", weight, x)
-    if bias is not None:
-        _check(name, "bias", bias, x)
-    if x.dtype == torch.float32:
-        raise RuntimeError(f"{name}: float32 is not supported (bfloat16 and float16 are); use torch.nn.functional.linear")
-    if x.dim() == 0 or weight.dim() != 2 or x.shape[-1] != weight.shape[1]:
-        raise RuntimeError(f"{name}: `x` {tuple(x.shape)} and `weight` {tuple(weight.shape)} do not match")
-    if bias is not None and bias.shape != weight.shape[:1]:
-        raise RuntimeError(f"{name}: `bias` {tuple(bias.shape)} does not match `weight` {tuple(weight.shape)}")
-    if saved is not None and (_rows(saved.shape), saved.shape[-1], saved.dtype, saved.device) != (_rows(x.shape), x.shape[-1], x.dtype, x.device):
-        raise RuntimeError(f"{name}: `saved` ({tuple(saved.shape)}, {saved.dtype}, {saved.device}) does not stand for `x` "
-                           f"({tuple(x.shape)}, {x.dtype}, {x.device})")  # fmt: skip
-    if not torch.is_grad_enabled():
-        return F.linear(x, weight, bias)
-    with torch.autocast("cuda", enabled=False):
-        return _Linear.apply(x, weight, bias, saved)
+    if saved is None:
+        return _lib.HOST.linear(x, weight, bias, (), (), None, None)
+    return _lib.HOST.linear(x, weight, bias, saved._tensors(), saved.shape, saved.dtype, saved.channel_scale)
 
 
 # ---------------------------------------------------------------------------------------------

@@ -1,4 +1,5 @@
-"""Builds the sm_100a kernel library in-tree: optimi_b200/lib/liboptimi_b200.so.
+"""Builds the sm_100a kernel library in-tree, optimi_b200/lib/liboptimi_b200.so, and beside it _host.so, the host side of
+optimi_b200/activations.py in C++ (autograd nodes and the calls of the library's C ABI; g++ and torch's headers).
 
     python -m optimi_b200.build [--force]
 
@@ -9,24 +10,33 @@ multiply-adds only where they say so with __fmaf_rn), default IEEE division and 
 from __future__ import annotations
 
 import hashlib
+import importlib.util
 import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 
 PKG = os.path.dirname(os.path.abspath(__file__))
 SRC = os.path.join(PKG, "csrc", "optimi_b200.cu")
 ACTIVATION_SRCS = [os.path.join(PKG, "csrc", "activation_ops.cu"), os.path.join(PKG, "csrc", "weight_gradient.cu")]
-DEPS = [SRC, os.path.join(PKG, "csrc", "mta_common.cuh"), os.path.join(PKG, "csrc", "optimizer_ops.cuh"),
+HOST_SRC = os.path.join(PKG, "csrc", "activations_host.cpp")
+DEPS = [SRC, HOST_SRC, os.path.join(PKG, "csrc", "mta_common.cuh"), os.path.join(PKG, "csrc", "optimizer_ops.cuh"),
         *ACTIVATION_SRCS, os.path.join(PKG, "csrc", "activation_common.cuh"),
         os.path.join(os.path.dirname(PKG), "include", "optimi_b200.h")]  # fmt: skip
 LIB_DIR = os.path.join(PKG, "lib")
 LIB = os.path.join(LIB_DIR, "liboptimi_b200.so")
+HOST_LIB = os.path.join(LIB_DIR, "_host.so")
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17", "-fmad=false", "-prec-div=true",
     "-prec-sqrt=true", "-ftz=false", "-Xcompiler", "-fPIC", "-Xcompiler", "-O2",
 ]  # fmt: skip
+
+
+def find_gxx() -> str:
+    """The system's compiler (the environment's CC and CXX may point at a wrapper)."""
+    return "/usr/bin/g++" if os.path.exists("/usr/bin/g++") else "g++"
 
 
 def find_nvcc() -> str:
@@ -36,12 +46,31 @@ def find_nvcc() -> str:
     raise RuntimeError("nvcc not found (set NVCC or add it to PATH)")
 
 
+def torch_dir() -> str:
+    """Where torch is installed (found without importing it)."""
+    return next(iter(importlib.util.find_spec("torch").submodule_search_locations))
+
+
+def host_compile(obj: str) -> list[str]:
+    torch, cuda = torch_dir(), os.path.dirname(os.path.dirname(os.path.realpath(find_nvcc())))
+    include = [os.path.join(torch, "include"), os.path.join(torch, "include", "torch", "csrc", "api", "include"),
+               sysconfig.get_paths()["include"], os.path.join(cuda, "include")]  # fmt: skip
+    return [find_gxx(), "-O2", "-std=c++17", "-fPIC", "-D_GLIBCXX_USE_CXX11_ABI=1", "-DTORCH_EXTENSION_NAME=_host", *[f"-I{d}" for d in include],
+            "-c", "-o", obj, HOST_SRC]  # fmt: skip
+
+
+def host_link(obj: str, lib: str, out: str) -> list[str]:
+    libs = os.path.join(torch_dir(), "lib")
+    return [find_gxx(), "-shared", "-o", out, obj, f"-L{libs}", "-lc10", "-lc10_cuda", "-ltorch", "-ltorch_cpu", "-ltorch_cuda", "-ltorch_python",
+            f"-L{os.path.dirname(lib)}", "-l:liboptimi_b200.so", "-Wl,-rpath,$ORIGIN"]  # fmt: skip
+
+
 STAMP = LIB + ".srchash"
 
 
 def source_hash() -> str:
     h = hashlib.sha256(" ".join(NVCC_FLAGS).encode())
-    for d in DEPS:
+    for d in [*DEPS, os.path.join(torch_dir(), "version.py")]:
         with open(d, "rb") as fh:
             h.update(fh.read())
     return h.hexdigest()
@@ -49,7 +78,7 @@ def source_hash() -> str:
 
 def up_to_date() -> bool:
     """True when the library was built from the sources as they are now (content hash, not mtime)."""
-    if not (os.path.exists(LIB) and os.path.exists(STAMP)):
+    if not (os.path.exists(LIB) and os.path.exists(HOST_LIB) and os.path.exists(STAMP)):
         return False
     with open(STAMP) as fh:
         return fh.read().strip() == source_hash()
@@ -73,7 +102,7 @@ def build(force: bool = False, verbose: bool = False) -> str:
         if not force and up_to_date():  # another process built it while this one waited
             return LIB
         nvcc = find_nvcc()
-        ccbin = ["-ccbin", "/usr/bin/g++"] if os.path.exists("/usr/bin/g++") else []  # the image's CC/CXX point at a wrapper
+        ccbin = ["-ccbin", find_gxx()]
         compile_flags = [f for f in NVCC_FLAGS if f not in ("-shared", "--use-local-env")]
         with tempfile.TemporaryDirectory(dir=LIB_DIR, prefix=".build-") as tmp:
             objs, procs = [], []
@@ -83,20 +112,25 @@ def build(force: bool = False, verbose: bool = False) -> str:
                 objs.append(obj)
                 cmd = [nvcc, *ccbin, *compile_flags, *(["-Xptxas", "-v"] if verbose else []), *defines, "-c", "-o", obj, src]
                 procs.append((cmd, subprocess.Popen(cmd, stdout=subprocess.PIPE, stderr=subprocess.PIPE, text=True)))
+            host_obj = os.path.join(tmp, "host.o")
+            cmd = host_compile(host_obj)
+            procs.append((cmd, subprocess.Popen(cmd, stdout=subprocess.PIPE, stderr=subprocess.PIPE, text=True)))
             log = ""
             for cmd, p in procs:
                 out, err = p.communicate()
                 log += out + err
                 if p.returncode != 0:
-                    raise RuntimeError("nvcc failed:\n" + " ".join(cmd) + "\n" + out + err)
+                    raise RuntimeError("compilation failed:\n" + " ".join(cmd) + "\n" + out + err)
             fresh = os.path.join(tmp, "liboptimi_b200.so")
-            link = [nvcc, *ccbin, "-shared", "-o", fresh, *objs]
-            res = subprocess.run(link, capture_output=True, text=True)
-            if res.returncode != 0:
-                raise RuntimeError("link failed:\n" + " ".join(link) + "\n" + res.stdout + res.stderr)
+            fresh_host = os.path.join(tmp, "_host.so")
+            for link in ([nvcc, *ccbin, "-shared", "-o", fresh, *objs], host_link(host_obj, fresh, fresh_host)):
+                res = subprocess.run(link, capture_output=True, text=True)
+                if res.returncode != 0:
+                    raise RuntimeError("link failed:\n" + " ".join(link) + "\n" + res.stdout + res.stderr)
             if os.path.exists(STAMP):
                 os.remove(STAMP)  # never a current stamp beside an older library
             os.replace(fresh, LIB)
+            os.replace(fresh_host, HOST_LIB)
         if verbose:
             print(log)
         with open(STAMP + ".tmp", "w") as fh:
