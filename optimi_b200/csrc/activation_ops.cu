@@ -219,6 +219,13 @@ __global__ void __launch_bounds__(kBlock) decompress_any_kernel(const int8_t* __
 template <typename T> struct Wide { using type = float; };
 template <> struct Wide<float> { using type = double; };
 
+// What the weight's gradient, a sum over all tokens, is added up in: for fp32 results 64 bits, as 60,000 terms of either sign leave
+// little more than five digits of a 32-bit sum.
+template <typename T> struct Total { using type = float; };
+template <> struct Total<float> { using type = double; };
+static __device__ __forceinline__ float add_product(float a, float b, float sum) { return __fmaf_rn(a, b, sum); }
+static __device__ __forceinline__ double add_product(float a, float b, double sum) { return __fma_rn((double)a, (double)b, sum); }
+
 // Sum over the P threads of a row, in all of them, added up in a fixed order.  `part` is this row's scratch; consecutive calls
 // alternate between two of them (turn), so that one barrier a call is enough.
 template <int P, typename F>
@@ -417,16 +424,17 @@ template <typename T, int P, int K, bool kAny>
 __global__ void __launch_bounds__(512, 1)
     rms_norm_backward_kernel(const T* __restrict__ grad, int64_t gs, const T* __restrict__ grad_sum, int64_t hs, const int8_t* __restrict__ codes,
                              int64_t pitch, const uint8_t* __restrict__ exponents, int64_t epitch, const float* __restrict__ rstd,
-                             const T* __restrict__ weight, int64_t rows, int cols, T* __restrict__ dx, float* __restrict__ lines,
-                             T* __restrict__ direct) {
+                             const T* __restrict__ weight, int64_t rows, int cols, T* __restrict__ dx,
+                             typename Total<T>::type* __restrict__ lines, T* __restrict__ direct) {
   using Values = Chunk<T>;
+  using A = typename Total<T>::type;
   constexpr bool kAhead = K <= 2;
   constexpr int C = Values::C, kThreads = 512, kGroups = kThreads / P;
   __shared__ float part[kGroups][2][P / 32];
-  __shared__ float sums[kGroups > 1 ? kGroups : 1][kGroups > 1 ? P * K * C + 4 : 1];
+  __shared__ A sums[kGroups > 1 ? kGroups : 1][kGroups > 1 ? P * K * C + 4 : 1];
   const int group = threadIdx.x / P, t = threadIdx.x % P;
   Values w[K];
-  float dw[K][C];
+  A dw[K][C];
   const auto weights = [&](int k) {
     const int c = (k * P + t) * C;
     Fetched<T, kAny> in;
@@ -437,7 +445,7 @@ __global__ void __launch_bounds__(512, 1)
   for (int k = 0; k < K; k++) {
     if constexpr (kAhead) w[k] = weights(k);
 #pragma unroll
-    for (int i = 0; i < C; i++) dw[k][i] = 0.0f;
+    for (int i = 0; i < C; i++) dw[k][i] = 0;
   }
   const int64_t step = (int64_t)gridDim.x * kGroups;
   const auto ask_sum = [&](int64_t row, BackwardRow<T, K, kAny>& v) {
@@ -482,7 +490,7 @@ __global__ void __launch_bounds__(512, 1)
 #pragma unroll
       for (int i = 0; i < C; i++) {
         const float n = v.code[k].get_scaled(i, unit, offset), d = g[k].get(i);
-        dw[k][i] = __fmaf_rn(d, n, dw[k][i]);
+        dw[k][i] = add_product(d, n, dw[k][i]);
         m = __fmaf_rn(weight ? __fmul_rn(d, wk.get(i)) : d, n, m);
       }
     }
@@ -521,7 +529,7 @@ __global__ void __launch_bounds__(512, 1)
       for (int i = 0; i < C; i++) {
         const int c = (k * P + t) * C + i;
         if (c >= cols) continue;
-        if (direct) direct[c] = from_f32<T>(dw[k][i]);
+        if (direct) direct[c] = from_f32<T>((float)dw[k][i]);
         else lines[(int64_t)blockIdx.x * cols + c] = dw[k][i];
       }
   } else {
@@ -531,10 +539,10 @@ __global__ void __launch_bounds__(512, 1)
       for (int i = 0; i < C; i++) sums[group][(k * P + t) * C + i] = dw[k][i];
     __syncthreads();
     for (int c = threadIdx.x; c < cols; c += kThreads) {
-      float s = sums[0][c];
+      A s = sums[0][c];
 #pragma unroll
       for (int j = 1; j < kGroups; j++) s += sums[j][c];
-      if (direct) direct[c] = from_f32<T>(s);
+      if (direct) direct[c] = from_f32<T>((float)s);
       else lines[(int64_t)blockIdx.x * cols + c] = s;
     }
   }
@@ -544,17 +552,17 @@ template <typename T>
 __global__ void long_rms_norm_backward_kernel(const T* __restrict__ grad, int64_t gs, const T* __restrict__ grad_sum, int64_t hs,
                                               const int8_t* __restrict__ codes, int64_t pitch, const uint8_t* __restrict__ exponents,
                                               int64_t epitch, const float* __restrict__ rstd, const T* __restrict__ weight, int64_t rows,
-                                              int64_t cols, T* __restrict__ dx, float* __restrict__ lines) {
-  float* line = lines ? lines + (int64_t)blockIdx.x * cols : nullptr;
+                                              int64_t cols, T* __restrict__ dx, typename Total<T>::type* __restrict__ lines) {
+  typename Total<T>::type* line = lines ? lines + (int64_t)blockIdx.x * cols : nullptr;
   if (line)
-    for (int64_t c = threadIdx.x; c < cols; c += blockDim.x) line[c] = 0.0f;
+    for (int64_t c = threadIdx.x; c < cols; c += blockDim.x) line[c] = 0;
   for (int64_t row = blockIdx.x; row < rows; row += gridDim.x) {
     float m = 0;
     for (int64_t c = threadIdx.x; c < cols; c += blockDim.x) {
       const float n = (float)codes[row * pitch + c] * power_of(exponents[row * epitch + c / kGroup]);
       const float g = to_f32(grad[row * gs + c]);
       m += (weight ? g * to_f32(weight[c]) : g) * n;
-      if (line) line[c] = __fmaf_rn(g, n, line[c]);
+      if (line) line[c] = add_product(g, n, line[c]);
     }
     if (!dx) continue;
     m = block_sum<float>(m) / (float)cols;
@@ -571,18 +579,20 @@ __global__ void long_rms_norm_backward_kernel(const T* __restrict__ grad, int64_
 
 // A warp of columns, 16 lines at a time; the 16 sums are added up in order.
 template <typename T>
-__global__ void __launch_bounds__(512) line_sum_kernel(const float* __restrict__ lines, int n_lines, int64_t cols, T* __restrict__ out) {
-  __shared__ float part[16][32];
+__global__ void __launch_bounds__(512) line_sum_kernel(const typename Total<T>::type* __restrict__ lines, int n_lines, int64_t cols,
+                                                       T* __restrict__ out) {
+  using A = typename Total<T>::type;
+  __shared__ A part[16][32];
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
   const int64_t c = (int64_t)blockIdx.x * 32 + lane;
-  float s = 0;
+  A s = 0;
   if (c < cols)
     for (int i = warp; i < n_lines; i += 16) s += lines[(int64_t)i * cols + c];
   part[warp][lane] = s;
   __syncthreads();
   if (warp != 0 || c >= cols) return;
   for (int i = 1; i < 16; i++) s += part[i][lane];
-  out[c] = from_f32<T>(s);
+  out[c] = from_f32<T>((float)s);
 }
 
 static inline unsigned grid_of(int64_t items, int64_t most) { return (unsigned)(items < most ? items : most); }
@@ -794,7 +804,7 @@ static unsigned backward_blocks(int64_t rows) { return grid_of(rows, kLongBlocks
 
 size_t optimi_b200_rms_norm_backward_workspace_bytes(int64_t rows, int64_t cols, int dtype) {
   if (rows <= 0 || cols <= 0 || !known_dtype(dtype) || one_block(rows, cols, dtype == OPTIMI_F32 ? 4 : 2)) return 0;
-  return (size_t)backward_blocks(rows) * (size_t)cols * sizeof(float);
+  return (size_t)backward_blocks(rows) * (size_t)cols * (dtype == OPTIMI_F32 ? sizeof(double) : sizeof(float));
 }
 
 int optimi_b200_rms_norm_backward(const void* grad, int64_t grad_stride, const void* grad_sum, int64_t grad_sum_stride,
@@ -822,14 +832,14 @@ int optimi_b200_rms_norm_backward(const void* grad, int64_t grad_stride, const v
                    !aligned(weight, 16) || !aligned(grad_input, 16);
   const Deal d = deal_of(cols, size, any ? kBackwardAnyChunks : kBackwardChunks);
   const bool alone = one_block(rows, cols, size);
-  float* lines = grad_weight && !alone ? (float*)workspace : nullptr;
+  void* lines = grad_weight && !alone ? workspace : nullptr;
   unsigned blocks = 0;
   FOR_DTYPE(dtype, {
     if (d.K == 0) {
       blocks = backward_blocks(rows);
       long_rms_norm_backward_kernel<T><<<blocks, 512, 0, s>>>((const T*)grad, grad_stride, (const T*)grad_sum, grad_sum_stride, (const int8_t*)codes,
                                                               code_pitch, (const uint8_t*)exponents, exponent_pitch, rstd, (const T*)weight,
-                                                              rows, cols, (T*)grad_input, lines);
+                                                              rows, cols, (T*)grad_input, (Total<T>::type*)lines);
     } else {
       const auto with_constants = [&](auto p, auto k, auto is_any) {
         constexpr int P = decltype(p)::value, K = decltype(k)::value;
@@ -837,7 +847,7 @@ int optimi_b200_rms_norm_backward(const void* grad, int64_t grad_stride, const v
         blocks = alone ? 1 : grid_of((rows + 512 / P - 1) / (512 / P), kBackwardBlocks);
         rms_norm_backward_kernel<T, P, K, kIsAny><<<blocks, 512, 0, s>>>(
             (const T*)grad, grad_stride, (const T*)grad_sum, grad_sum_stride, (const int8_t*)codes, code_pitch, (const uint8_t*)exponents,
-            exponent_pitch, rstd, (const T*)weight, rows, (int)cols, (T*)grad_input, lines, alone ? (T*)grad_weight : nullptr);
+            exponent_pitch, rstd, (const T*)weight, rows, (int)cols, (T*)grad_input, (typename Total<T>::type*)lines, alone ? (T*)grad_weight : nullptr);
       };
       if (any) with_deal<T, kBackwardAnyChunks>(d, [&](auto p, auto k) { with_constants(p, k, std::true_type()); });
       else with_deal<T, kBackwardChunks>(d, [&](auto p, auto k) { with_constants(p, k, std::false_type()); });
@@ -845,7 +855,7 @@ int optimi_b200_rms_norm_backward(const void* grad, int64_t grad_stride, const v
   });
   rc = launched(fn);
   if (rc != OPTIMI_OK || !lines) return rc;
-  FOR_DTYPE(dtype, (line_sum_kernel<T><<<(unsigned)((cols + 31) / 32), 512, 0, s>>>(lines, (int)blocks, cols, (T*)grad_weight)));
+  FOR_DTYPE(dtype, (line_sum_kernel<T><<<(unsigned)((cols + 31) / 32), 512, 0, s>>>((const Total<T>::type*)lines, (int)blocks, cols, (T*)grad_weight)));
   return launched(fn);
 }
 

@@ -243,6 +243,21 @@ def test_norm_variants(shape, dtype, variant):
     check_norm(loud(shape, dtype, 1), w, r, normal(shape, dtype, 3, 0.1), dh)
 
 
+@pytest.mark.parametrize("channels", [1, 17, 64, 9000])
+def test_norm_weight_gradient_of_many_tokens_keeps_its_digits(channels):
+    """float32: terms of either sign all but cancel; added up in 64 bits and rounded once, the result is off by half a step of itself."""
+    tokens = 60_000 if channels < 1000 else 3000
+    x, dy = normal((tokens, channels), torch.float32, 1).cuda().requires_grad_(), normal((tokens, channels), torch.float32, 2).cuda()
+    w = torch.ones(channels, device="cuda").requires_grad_()
+    out = act().rms_norm(x, w, eps=EPS)
+    (dw,) = torch.autograd.grad(out.output, w, dy)
+    v = out.saved.decompress().double()
+    want = (dy.double() * v).sum(dim=0)
+    # 64-bit sums are off by at most tokens * 2^-53 of the sum of magnitudes, here 7e-12
+    slack = (dy.double() * v).abs().sum(dim=0) * tokens * 2.0**-53
+    assert bool(((dw.double() - want).abs() <= want.abs() * U32 + slack * 2).all())
+
+
 @pytest.mark.parametrize("dtype", DTYPES, ids=name_of)
 def test_norm_strides(dtype):
     base, other = loud((40, 3, 160), dtype, 1).cuda(), normal((40, 3, 160), dtype, 2).cuda()
@@ -959,3 +974,9 @@ def test_offsets_beyond_32_bits():
     some[2:-2] = 0
     few = a.CompressedActivation(saved.codes[keep], saved.exponents[keep], (4, cols), torch.bfloat16)
     check_weight_gradient(some[keep], few, a.weight_gradient(some, saved))
+    del x, xg, xt, saved, some, grad
+    # a result of more than 2^31 values: its last rows are those of the last outputs taken alone
+    dy, kept = normal((16, 70_008), torch.bfloat16, 6).cuda(), a.compress(normal((16, cols), torch.bfloat16, 7).cuda())
+    dw = a.weight_gradient(dy, kept)
+    assert dw.numel() > 2**31
+    check_weight_gradient(dy[:, -8:].contiguous(), kept, dw[-8:])
