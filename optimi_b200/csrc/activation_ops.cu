@@ -250,6 +250,21 @@ static __device__ __forceinline__ void store_chunk(const Chunk<T>& v, T* row, in
   else if (c < cols) v.store(row + c);
 }
 
+// A chunk of the weight; ones where there is none, so that the loops over values ask nothing.
+template <typename T, bool kAny>
+static __device__ __forceinline__ Chunk<T> weight_chunk(const T* weight, int c, int cols) {
+  Chunk<T> v;
+  if (weight) {
+    Fetched<T, kAny> in;
+    in.fetch(weight + c, cols - c);
+    v = in.settle(weight + c, cols - c);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; i++) v.w[i] = std::is_same<T, float>::value ? 0x3f800000u : std::is_same<T, __half>::value ? 0x3c003c00u : 0x3f803f80u;
+  }
+  return v;
+}
+
 template <typename T, int P, int K, bool kAny, bool kKeep>
 __global__ void __launch_bounds__(P < 128 ? 128 : P, kAny && K <= 2 ? 1024 / (P < 128 ? 128 : P) : 0)
     rms_norm_kernel(const T* __restrict__ x, int64_t xs, const T* __restrict__ residual, int64_t rs, const T* __restrict__ weight,
@@ -262,15 +277,8 @@ __global__ void __launch_bounds__(P < 128 ? 128 : P, kAny && K <= 2 ? 1024 / (P 
   const int group = threadIdx.x / P, t = threadIdx.x % P;
   const int padded = (cols + kGroup - 1) / kGroup * kGroup;
   Values w[K];
-  if (weight) {
 #pragma unroll
-    for (int k = 0; k < K; k++) {
-      const int c = (k * P + t) * C;
-      Fetched<T, kAny> in;
-      in.fetch(weight + c, cols - c);
-      w[k] = in.settle(weight + c, cols - c);
-    }
-  }
+  for (int k = 0; k < K; k++) w[k] = weight_chunk<T, kAny>(weight, (k * P + t) * C, cols);
   int turn = 0;
   for (int64_t row = (int64_t)blockIdx.x * kGroups + group; row < rows; row += (int64_t)gridDim.x * kGroups, turn++) {
     Values h[K];
@@ -334,7 +342,7 @@ __global__ void __launch_bounds__(P < 128 ? 128 : P, kAny && K <= 2 ? 1024 / (P 
 #pragma unroll
       for (int i = 0; i < C; i++) {
         n[i] = (F)h[k].get(i) * rstd;
-        f[i] = (float)(weight ? n[i] * (F)w[k].get(i) : n[i]);
+        f[i] = (float)(n[i] * (F)w[k].get(i));
       }
       Values out;
       out.set(f);
@@ -435,12 +443,7 @@ __global__ void __launch_bounds__(512, 1)
   const int group = threadIdx.x / P, t = threadIdx.x % P;
   Values w[K];
   A dw[K][C];
-  const auto weights = [&](int k) {
-    const int c = (k * P + t) * C;
-    Fetched<T, kAny> in;
-    in.fetch(weight + c, weight ? cols - c : 0);
-    return in.settle(weight + c, weight ? cols - c : 0);
-  };
+  const auto weights = [&](int k) { return weight_chunk<T, kAny>(weight, (k * P + t) * C, cols); };
 #pragma unroll
   for (int k = 0; k < K; k++) {
     if constexpr (kAhead) w[k] = weights(k);
@@ -491,7 +494,7 @@ __global__ void __launch_bounds__(512, 1)
       for (int i = 0; i < C; i++) {
         const float n = v.code[k].get_scaled(i, unit, offset), d = g[k].get(i);
         dw[k][i] = add_product(d, n, dw[k][i]);
-        m = __fmaf_rn(weight ? __fmul_rn(d, wk.get(i)) : d, n, m);
+        m = __fmaf_rn(__fmul_rn(d, wk.get(i)), n, m);
       }
     }
     if (dx) {
@@ -502,15 +505,14 @@ __global__ void __launch_bounds__(512, 1)
       for (int k = 0; k < K; k++) {
         const int c = (k * P + t) * C;
         const float unit = power_of((int)v.e[k]), offset = v.code[k].scaled_offset(unit);
-        Values wk, s;
+        Values wk;
         if constexpr (kAhead) wk = w[k];
         else wk = weights(k);
-        if (grad_sum) s = v.s[k].settle(grad_sum + row * hs + c, cols - c);
+        const Values s = v.s[k].settle(grad_sum + row * hs + c, cols - c);  // zeros where there is none
         float f[C];
 #pragma unroll
         for (int i = 0; i < C; i++) {  // rstd * g + dsum, then - xn * (m * rstd)
-          const float d = weight ? __fmul_rn(g[k].get(i), wk.get(i)) : g[k].get(i);
-          f[i] = grad_sum ? __fmaf_rn(v.r, d, s.get(i)) : __fmul_rn(v.r, d);
+          f[i] = __fmaf_rn(v.r, __fmul_rn(g[k].get(i), wk.get(i)), s.get(i));
           f[i] = __fmaf_rn(v.code[k].get_scaled(i, unit, offset), mr, f[i]);
         }
         Values out;

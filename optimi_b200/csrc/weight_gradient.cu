@@ -119,9 +119,10 @@ static __device__ __forceinline__ void multiply(uint32_t d, uint32_t a, uint64_t
 }
 
 // What the pairs of blocks do.  (A block per tile, started anew for each, lost 9 us a tile to its start and to storing results: the
-// pairs stay, and results are stored while the next tile is multiplied.)  `whole` tiles are dealt out in turns, all their tokens at once, so that the pairs of one turn
-// read the same tokens at the same time (from L2); the tiles that would not fill another turn are cut into `slices` along
-// the tokens, whose sums go to the workspace in fp32 and are added up in order by a second kernel.
+// pairs stay, and results are stored while the next tile is multiplied.)  `whole` tiles are dealt out in turns, all their
+// tokens at once, so that the pairs of one turn read the same tokens at the same time (from L2); the tiles that would not
+// fill another turn are cut into `slices` along the tokens, whose sums go to the workspace in fp32 and are added up in order
+// by a second kernel.
 struct Plan {
   int rows, outputs, channels;
   int steps;         // of kK tokens
