@@ -10,9 +10,13 @@ namespace act {
 // Both stream: an item is a chunk of C values in one thread (the neighbouring lanes of a group find its largest magnitude
 // together), kUnroll items a thread are loaded before the first is used, and nothing is read or written twice.  Bound by HBM:
 // 8192 x 14336 bf16 stored and restored in 112 us, 6.3 TB/s (0.98 of the measured copy rate); a warp to a group with one value a lane
-// took 688 us.  Rows of odd width spend their time on shifting: 4096 x 4095 bf16 20 and 25 us, 4096 x 4096 under 13 each.
+// took 688 us.  Rows of odd width spend their time on shifting: 4096 x 4095 bf16 19 us each way, 4096 x 4096 under 13.
 constexpr int kBlock = 256, kUnroll = 4;
 
+static __device__ __forceinline__ void divide(int a, int b, int* quotient, int* rest) {
+  *quotient = (uint32_t)a / (uint32_t)b;
+  *rest = (uint32_t)a % (uint32_t)b;
+}
 static __device__ __forceinline__ void divide(int64_t a, int64_t b, int64_t* quotient, int64_t* rest) {
   if (((a | b) >> 31) == 0) {
     *quotient = (uint32_t)a / (uint32_t)b;
@@ -23,11 +27,13 @@ static __device__ __forceinline__ void divide(int64_t a, int64_t b, int64_t* quo
   }
 }
 
-// The rows and columns (in units of `per_row` a row) of the items that a thread takes: one division, then steps of kBlock items.
+// The rows and columns (in units of `per_row` a row) of the items that a thread takes: one division, then steps of kBlock items.  I:
+// int where all offsets fit, else 64 bits (4096 x 4095 bf16 restored: 18.5 us, 26.7 with 64 bits).
+template <typename I>
 struct Walk {
-  int64_t row, col;
-  int64_t rows_on, cols_on, per_row;
-  __device__ __forceinline__ Walk(int64_t item, int64_t step, int64_t units_per_row) : per_row(units_per_row) {
+  I row, col;
+  I rows_on, cols_on, per_row;
+  __device__ __forceinline__ Walk(I item, I step, I units_per_row) : per_row(units_per_row) {
     divide(item, per_row, &row, &col);
     divide(step, per_row, &rows_on, &cols_on);
   }
@@ -41,22 +47,21 @@ struct Walk {
 // long row and nothing is divided.  kRows: every row begins on 16 bytes and is whole chunks.  kAny: neither.
 enum Lie : int { kFlat, kRows, kAny };
 
-template <typename T, int kLie>
-__global__ void __launch_bounds__(kBlock) compress_kernel(const T* __restrict__ x, int64_t items, int64_t chunks, int64_t cols, int64_t stride,
-                                                          int8_t* __restrict__ codes, int64_t pitch, uint8_t* __restrict__ exponents,
-                                                          int64_t epitch) {
+template <typename T, int kLie, typename I>
+__global__ void __launch_bounds__(kBlock) compress_kernel(const T* __restrict__ x, I items, I chunks, I cols, I stride, int8_t* __restrict__ codes,
+                                                          I pitch, uint8_t* __restrict__ exponents, I epitch) {
   constexpr int C = Chunk<T>::C, kLanes = Chunk<T>::kLanes;
-  const int64_t first = (int64_t)blockIdx.x * (kBlock * kUnroll) + threadIdx.x;
+  const I first = (I)blockIdx.x * (kBlock * kUnroll) + threadIdx.x;
   Fetched<T, kLie == kAny> in[kUnroll];
-  int64_t row[kUnroll], col[kUnroll];
+  I row[kUnroll], col[kUnroll];
   int n[kUnroll];
-  Walk walk(kLie == kFlat ? 0 : first, kBlock, kLie == kFlat ? 1 : chunks);
+  Walk<I> walk(kLie == kFlat ? 0 : first, kBlock, kLie == kFlat ? 1 : chunks);
 #pragma unroll
   for (int u = 0; u < kUnroll; u++) {
-    const int64_t item = first + u * kBlock;
+    const I item = first + u * kBlock;
     row[u] = kLie == kFlat ? 0 : walk.row, col[u] = (kLie == kFlat ? item : walk.col) * C;
     if (kLie != kFlat) walk.on();
-    n[u] = item >= items ? 0 : kLie == kFlat ? C : (int)min((int64_t)C, cols - col[u]);
+    n[u] = item >= items ? 0 : kLie == kFlat ? C : (int)min((I)C, cols - col[u]);
     in[u].fetch(x + row[u] * stride + col[u], n[u]);
   }
 #pragma unroll
@@ -84,7 +89,7 @@ __global__ void __launch_bounds__(kBlock) decompress_kernel(const int8_t* __rest
   CodeChunk<C> c[kUnroll];
   uint32_t e[kUnroll];
   int64_t row[kUnroll], col[kUnroll];
-  Walk walk(kLie == kFlat ? 0 : first, kBlock, kLie == kFlat ? 1 : chunks);
+  Walk<int64_t> walk(kLie == kFlat ? 0 : first, kBlock, kLie == kFlat ? 1 : chunks);
 #pragma unroll
   for (int u = 0; u < kUnroll; u++) {
     const int64_t item = first + u * kBlock;
@@ -129,7 +134,7 @@ __global__ void __launch_bounds__(kBlock) align_rows_kernel(const T* __restrict_
   Fetched<T, true> in[kUnroll];
   const T* from[kUnroll];
   int n[kUnroll];
-  Walk walk(first, kBlock, chunks);
+  Walk<int64_t> walk(first, kBlock, chunks);
 #pragma unroll
   for (int u = 0; u < kUnroll; u++, walk.on()) {
     from[u] = x + walk.row * stride + walk.col * C;
@@ -143,16 +148,16 @@ __global__ void __launch_bounds__(kBlock) align_rows_kernel(const T* __restrict_
 
 // decompress for rows that begin anywhere.  The result has no gaps, so an item is one 16-byte block of it as a whole; its codes lie at
 // any byte of a row (whose pitch is a multiple of 32), and a block that reaches into the next row takes them one by one.
-template <typename T, bool kScaled>
-__global__ void __launch_bounds__(kBlock) decompress_any_kernel(const int8_t* __restrict__ codes, int64_t pitch, const uint8_t* __restrict__ exponents,
-                                                                int64_t epitch, const T* __restrict__ channel_scale, int64_t values,
-                                                                int64_t cols, T* __restrict__ out) {
+template <typename T, bool kScaled, typename I>
+__global__ void __launch_bounds__(kBlock) decompress_any_kernel(const int8_t* __restrict__ codes, I pitch, const uint8_t* __restrict__ exponents,
+                                                                I epitch, const T* __restrict__ channel_scale, I values, I cols,
+                                                                T* __restrict__ out) {
   constexpr int C = Chunk<T>::C;
-  const int64_t first = (int64_t)blockIdx.x * (kBlock * kUnroll) + threadIdx.x;
+  const I first = (I)blockIdx.x * (kBlock * kUnroll) + threadIdx.x;
   uint32_t w[kUnroll][C / 4 + 1];
   uint32_t low[kUnroll], high[kUnroll];
-  int64_t col[kUnroll];
-  Walk walk(first * C, kBlock * C, cols);
+  I col[kUnroll];
+  Walk<I> walk(first * C, kBlock * C, cols);
 #pragma unroll
   for (int u = 0; u < kUnroll; u++, walk.on()) {
     col[u] = walk.col;
@@ -160,7 +165,7 @@ __global__ void __launch_bounds__(kBlock) decompress_any_kernel(const int8_t* __
     for (int i = 0; i <= C / 4; i++) w[u][i] = 0;
     low[u] = high[u] = 0;
     if ((first + u * kBlock) * C < values && walk.col + C <= cols) {
-      const uint32_t* words = reinterpret_cast<const uint32_t*>(codes + walk.row * pitch + (walk.col & ~3ll));
+      const uint32_t* words = reinterpret_cast<const uint32_t*>(codes + walk.row * pitch + (walk.col & ~(I)3));
 #pragma unroll
       for (int i = 0; i < C / 4; i++) w[u][i] = words[i];
       if (walk.col & 3) w[u][C / 4] = words[C / 4];  // the last code asked for lies there
@@ -170,7 +175,7 @@ __global__ void __launch_bounds__(kBlock) decompress_any_kernel(const int8_t* __
   }
 #pragma unroll
   for (int u = 0; u < kUnroll; u++) {
-    const int64_t at = (first + u * kBlock) * C;
+    const I at = (first + u * kBlock) * C;
     if (at >= values) return;
     float f[C];
     if (col[u] + C <= cols) {
@@ -183,7 +188,7 @@ __global__ void __launch_bounds__(kBlock) decompress_any_kernel(const int8_t* __
     } else {
 #pragma unroll
       for (int i = 0; i < C; i++) {
-        int64_t r, k;
+        I r, k;
         divide(min(at + i, values - 1), cols, &r, &k);
         f[i] = __fmul_rn((float)codes[r * pitch + k], power_of(exponents[r * epitch + k / kGroup]));
       }
@@ -661,6 +666,12 @@ static int check_shape(const char* fn, int64_t rows, int64_t cols, int dtype) {
   return OPTIMI_OK;
 }
 
+// Whether offsets into rows `stride` and `pitch` apart, and the items a last block reaches past the end, fit 32 bits.
+static bool small_offsets(int64_t rows, int64_t stride, int64_t pitch) {
+  const int64_t most = (1ll << 31) - (1 << 20);
+  return rows * pitch < most && rows * stride < most;
+}
+
 template <typename T>
 static void launch_compress(const void* x, int64_t stride, int64_t rows, int64_t cols, void* codes, int64_t pitch, void* exponents,
                             int64_t epitch, cudaStream_t s) {
@@ -669,11 +680,13 @@ static void launch_compress(const void* x, int64_t stride, int64_t rows, int64_t
   const bool regular = cols % C == 0 && rows_aligned(x, stride, rows, sizeof(T));
   const bool flat = regular && cols % kGroup == 0 && (rows == 1 || (stride == cols && pitch == cols && epitch * kGroup == cols));
   const unsigned blocks = (unsigned)((items + kBlock * kUnroll - 1) / (kBlock * kUnroll));
-#define LAUNCH(lie)                                                                                                             \
-  compress_kernel<T, lie><<<blocks, kBlock, 0, s>>>((const T*)x, items, chunks, cols, stride, (int8_t*)codes, pitch, (uint8_t*)exponents, epitch)
-  if (flat) LAUNCH(kFlat);
-  else if (regular) LAUNCH(kRows);
-  else LAUNCH(kAny);
+#define LAUNCH(lie, I)                                                                                                             \
+  compress_kernel<T, lie, I><<<blocks, kBlock, 0, s>>>((const T*)x, (I)items, (I)chunks, (I)cols, (I)stride, (int8_t*)codes, (I)pitch, \
+                                                       (uint8_t*)exponents, (I)epitch)
+  if (flat) LAUNCH(kFlat, int64_t);
+  else if (regular) LAUNCH(kRows, int64_t);
+  else if (small_offsets(rows, stride, pitch)) LAUNCH(kAny, int);
+  else LAUNCH(kAny, int64_t);
 #undef LAUNCH
 }
 
@@ -690,9 +703,12 @@ static void launch_decompress(const void* codes, int64_t pitch, const void* expo
                                                                (const T*)scale, items, chunks, cols, (T*)out)
   if (flat) LAUNCH(kFlat);
   else if (regular) LAUNCH(kRows);
+  else if (small_offsets(rows, cols, pitch))
+    decompress_any_kernel<T, kScaled, int><<<blocks, kBlock, 0, s>>>((const int8_t*)codes, (int)pitch, (const uint8_t*)exponents, (int)epitch,
+                                                                     (const T*)scale, (int)(rows * cols), (int)cols, (T*)out);
   else
-    decompress_any_kernel<T, kScaled><<<blocks, kBlock, 0, s>>>((const int8_t*)codes, pitch, (const uint8_t*)exponents, epitch, (const T*)scale,
-                                                                rows * cols, cols, (T*)out);
+    decompress_any_kernel<T, kScaled, int64_t><<<blocks, kBlock, 0, s>>>((const int8_t*)codes, pitch, (const uint8_t*)exponents, epitch,
+                                                                         (const T*)scale, rows * cols, cols, (T*)out);
 #undef LAUNCH
 }
 

@@ -954,6 +954,12 @@ def test_offsets_beyond_32_bits():
     back = a.decompress(saved)
     assert same_bits(back[-5:], a.decompress(tail))
     del back
+    odd = a.compress(x[:, 1:])  # rows that begin anywhere
+    tail = a.compress(x[-5:, 1:].contiguous())
+    assert torch.equal(odd.codes[-5:], tail.codes) and torch.equal(odd.exponents[-5:], tail.exponents)
+    back = a.decompress(odd)
+    assert same_bits(back[-5:], a.decompress(tail))
+    del back, odd
     w = torch.ones(cols, dtype=torch.bfloat16, device="cuda")
     xg = x.requires_grad_()
     out = a.rms_norm(xg, w)
