@@ -677,6 +677,51 @@ def test_prepared_model_under_autocast():
     assert abs(float(loss_of(twin, idx)) - float(loss_of(model, idx))) < 7e-5
 
 
+@pytest.mark.parametrize("through", ["torch", "8 bits"])
+def test_prepared_model_recomputed_in_the_backward_pass(through):
+    """Recomputation makes the same kept rows again: the gradients of the prepared model, bit for bit where the block's input is
+    kept as it is."""
+    import optimi_b200
+
+    idx = torch.randint(0, 200, (8, 64), device="cuda", generator=torch.Generator(device="cuda").manual_seed(1))
+    model = optimi_b200.prepare_for_compressed_activations(decoder())
+    loss_of(model, idx).backward()
+    want = {n: p.grad.clone() for n, p in model.named_parameters()}
+    model.zero_grad()
+    if through == "torch":
+        loss_of(model, idx, through=lambda b, x: torch.utils.checkpoint.checkpoint(b, x, use_reentrant=False)).backward()
+    else:
+        loss_of(model, idx, through=act().checkpoint).backward()
+    for n, p in model.named_parameters():
+        if through == "torch":
+            # (an embedding's gradient is a scatter of additions in no fixed order)
+            assert same_bits(p.grad, want[n]) or "embed" in n and relative(p.grad, want[n]) < 1e-5, n
+        else:
+            assert relative(p.grad, want[n]) < 0.05, n
+
+
+def test_prepared_norm_without_weight_and_copies_of_a_prepared_model():
+    import io
+
+    import optimi_b200
+
+    model = nn.Sequential(nn.RMSNorm(64, elementwise_affine=False), nn.Linear(64, 32)).to(device="cuda", dtype=torch.bfloat16)
+    optimi_b200.prepare_for_compressed_activations(model)
+    x, dy = normal((40, 64), torch.bfloat16, 1).cuda().requires_grad_(), normal((40, 32), torch.bfloat16, 2).cuda()
+    want = torch.autograd.grad(model(x), [x, *model.parameters()], dy)
+    out = act().rms_norm(x)
+    assert same_bits(want[1], act().weight_gradient(dy, out.saved))
+    buf = io.BytesIO()
+    torch.save(model, buf)
+    buf.seek(0)
+    for twin in (copy.deepcopy(model), torch.load(buf, weights_only=False)):
+        for a, b in zip(torch.autograd.grad(twin(x), [x, *twin.parameters()], dy), want):
+            assert same_bits(a, b)
+        optimi_b200.remove_compressed_activations(twin)
+        assert type(twin[0]) is nn.RMSNorm and type(twin[1]) is nn.Linear
+    assert type(model[1]) is not nn.Linear
+
+
 def test_a_norm_output_that_was_written_to_is_not_mistaken_for_the_kept_one():
     import optimi_b200
 
