@@ -244,11 +244,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         __syncwarp();
       }
     }
-    // Nothing of a block's shared memory is given back while a copy into it is under way: both blocks wait for the codes they
-    // asked for, the first for the gradients of both.  (The partner stays until the first block is here too.)
+    // Nothing of a block's shared memory is given back while a copy into it or an arrival there is under way: both blocks wait for the
+    // codes they asked for, the first for the gradients of both (the partner stays until the first block is here too), and both for
+    // the multiplications' arrivals at their own barriers, which the barrier of the pair does not order.
     for (int n = g > kStages ? g - kStages : 0; n < g; n++) {
       ok &= barrier_wait(codes_in + 8 * (n % kStages), (n / kStages) & 1);
       if (half == 0) ok &= barrier_wait(grads_in + 8 * (n % kStages), (n / kStages) & 1);
+      ok = ok && barrier_wait(empty + 8 * (n % kStages), (n / kStages) & 1);
     }
   } else if (warp == kIssuer) {
     if (half == 0) {
@@ -422,6 +424,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       }
 #undef LOAD16
     }
+    ok &= barrier_wait(drained, 0);  // the last arrival in this block, as above
   }
   if (!ok) g_gave_up = 1;
   __syncwarp();
