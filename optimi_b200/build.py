@@ -22,7 +22,7 @@ SRC = os.path.join(PKG, "csrc", "optimi_b200.cu")
 ACTIVATION_SRCS = [os.path.join(PKG, "csrc", "activation_ops.cu"), os.path.join(PKG, "csrc", "weight_gradient.cu")]
 HOST_SRC = os.path.join(PKG, "csrc", "activations_host.cpp")
 DEPS = [SRC, HOST_SRC, os.path.join(PKG, "csrc", "mta_common.cuh"), os.path.join(PKG, "csrc", "optimizer_ops.cuh"),
-        *ACTIVATION_SRCS, os.path.join(PKG, "csrc", "activation_common.cuh"),
+        *ACTIVATION_SRCS, os.path.join(PKG, "csrc", "activation_common.cuh"), os.path.join(PKG, "csrc", "activation_offsets.h"),
         os.path.join(os.path.dirname(PKG), "include", "optimi_b200.h")]  # fmt: skip
 LIB_DIR = os.path.join(PKG, "lib")
 LIB = os.path.join(LIB_DIR, "liboptimi_b200.so")

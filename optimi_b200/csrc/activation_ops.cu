@@ -1,5 +1,6 @@
 // Activations kept in 8 bits (format: activation_common.cuh) and the RMS norm that writes and reads them.
 #include "activation_common.cuh"
+#include "activation_offsets.h"
 
 namespace optimi {
 namespace act {
@@ -666,12 +667,6 @@ static int check_shape(const char* fn, int64_t rows, int64_t cols, int dtype) {
   return OPTIMI_OK;
 }
 
-// Whether offsets into rows `stride` and `pitch` apart, and the items a last block reaches past the end, fit 32 bits.
-static bool small_offsets(int64_t rows, int64_t stride, int64_t pitch) {
-  const int64_t most = (1ll << 31) - (1 << 20);
-  return rows * pitch < most && rows * stride < most;
-}
-
 template <typename T>
 static void launch_compress(const void* x, int64_t stride, int64_t rows, int64_t cols, void* codes, int64_t pitch, void* exponents,
                             int64_t epitch, cudaStream_t s) {
@@ -685,7 +680,7 @@ static void launch_compress(const void* x, int64_t stride, int64_t rows, int64_t
                                                        (uint8_t*)exponents, (I)epitch)
   if (flat) LAUNCH(kFlat, int64_t);
   else if (regular) LAUNCH(kRows, int64_t);
-  else if (small_offsets(rows, stride, pitch)) LAUNCH(kAny, int);
+  else if (small_offsets(rows, stride, pitch, epitch)) LAUNCH(kAny, int);
   else LAUNCH(kAny, int64_t);
 #undef LAUNCH
 }
@@ -703,7 +698,7 @@ static void launch_decompress(const void* codes, int64_t pitch, const void* expo
                                                                (const T*)scale, items, chunks, cols, (T*)out)
   if (flat) LAUNCH(kFlat);
   else if (regular) LAUNCH(kRows);
-  else if (small_offsets(rows, cols, pitch))
+  else if (small_offsets(rows, cols, pitch, epitch))
     decompress_any_kernel<T, kScaled, int><<<blocks, kBlock, 0, s>>>((const int8_t*)codes, (int)pitch, (const uint8_t*)exponents, (int)epitch,
                                                                      (const T*)scale, (int)(rows * cols), (int)cols, (T*)out);
   else

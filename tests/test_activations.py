@@ -2,6 +2,8 @@
 
 import copy
 import ctypes
+import os
+import subprocess
 import warnings
 
 import pytest
@@ -156,3 +158,35 @@ def test_workspaces_grow_with_the_problem():
     assert L.optimi_b200_rms_norm_backward_workspace_bytes(1, 64, 1) == 0  # one block adds up the rows itself
     assert 0 < L.optimi_b200_rms_norm_backward_workspace_bytes(100, 64, 1) < L.optimi_b200_rms_norm_backward_workspace_bytes(1000, 64, 1)
     assert L.optimi_b200_rms_norm_backward_workspace_bytes(1000, 64, 9) == 0
+
+
+@pytest.fixture(scope="module")
+def small_offsets(tmp_path_factory):
+    """The choice between offsets of 32 and 64 bits, from the header the kernels' launches include, through the host's compiler."""
+    where = tmp_path_factory.mktemp("offsets")
+    source, lib = where / "offsets.cpp", where / "offsets.so"
+    header = os.path.join(os.path.dirname(optimi_b200.__file__), "csrc", "activation_offsets.h")
+    source.write_text(f'#include "{header}"\nextern "C" int small(int64_t r, int64_t s, int64_t p, int64_t e) {{ return optimi::act::small_offsets(r, s, p, e); }}\n')
+    subprocess.run([_lib._build.find_gxx(), "-std=c++17", "-shared", "-fPIC", "-o", str(lib), str(source)], check=True)
+    fn = ctypes.CDLL(str(lib)).small
+    fn.argtypes = [ctypes.c_int64] * 4
+    return lambda *args: bool(fn(*args))
+
+
+def test_offsets_of_32_bits_only_where_all_of_them_fit(small_offsets):
+    assert small_offsets(4096, 4095, 4096, 128) and small_offsets(1, 1, 32, 1)
+    assert small_offsets(70_000, 31, 32, 29_000)  # 2.03e9 bytes of exponents from the first row to the last
+    # exponents that are columns of a wide table: rows 32 KB apart reach past 2^31
+    assert not small_offsets(70_000, 31, 32, 32_768) and not small_offsets(65_536, 31, 32, 32_768)
+    assert not small_offsets(70_000, 32_767, 32, 1) and not small_offsets(70_000, 31, 32_768, 1)
+    for at in range(3):
+        steps = [1, 32, 1]
+        steps[at] = 1 << 62  # the product would not fit 64 bits
+        assert not small_offsets(1 << 30, *steps)
+    # and never where an offset of the last row reaches 2^31
+    for rows in (1, 2, 3, 1000, 65_537, (1 << 31) - 1):
+        for step in (1, 31, (1 << 31) // rows - 1, (1 << 31) // rows, (1 << 31) // rows + 1):
+            for at in range(3):
+                steps = [1, 1, 1]
+                steps[at] = step
+                assert not small_offsets(rows, *steps) or rows * step < 1 << 31

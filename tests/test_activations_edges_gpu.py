@@ -37,3 +37,16 @@ def test_weight_gradients_one_behind_another():
         for grad, saved, want in calls:
             wrong += (a.weight_gradient(grad, saved) != want).sum()
     assert int(wrong) == 0 and gave_up() == 0
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "fp32"])
+def test_exponents_that_are_columns_of_a_table_beyond_32_bits(dtype):
+    """Codes close together and exponents 32 KB from row to row: the last rows' lie beyond 2^31 bytes."""
+    a = act()
+    rows, cols = 70_000, 31
+    x = torch.randn((rows, cols), generator=torch.Generator(device="cuda").manual_seed(1), device="cuda").to(dtype)
+    dense = a.compress(x)
+    table = torch.zeros((rows, 32_768), dtype=torch.uint8, device="cuda")
+    table[:, 5:6] = dense.exponents
+    wide = a.CompressedActivation(dense.codes, table[:, 5:6], (rows, cols), dtype)
+    assert torch.equal(wide.decompress(), dense.decompress())
