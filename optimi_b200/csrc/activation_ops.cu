@@ -838,8 +838,9 @@ int optimi_b200_rms_norm_backward(const void* grad, int64_t grad_stride, const v
   rc = check_codes(fn, codes, code_pitch, exponents, exponent_pitch, cols);
   if (rc != OPTIMI_OK) return rc;
   const size_t need = optimi_b200_rms_norm_backward_workspace_bytes(rows, cols, dtype);
-  if (grad_weight && need > 0 && (!workspace || workspace_bytes < need))
-    return fail(OPTIMI_ERR_WORKSPACE_TOO_SMALL, "%s: workspace has %zu bytes, %zu are needed", fn, workspace ? workspace_bytes : (size_t)0, need);
+  if (grad_weight && need > 0 && (!workspace || workspace_bytes < need || !aligned(workspace, 16)))
+    return fail(OPTIMI_ERR_WORKSPACE_TOO_SMALL, "%s: workspace has %zu bytes, %zu are needed, 16-byte aligned", fn,
+                workspace ? workspace_bytes : (size_t)0, need);
   const int size = dtype == OPTIMI_F32 ? 4 : 2;
   const bool any = cols * size % 16 || !rows_aligned(grad, grad_stride, rows, size) || (grad_sum && !rows_aligned(grad_sum, grad_sum_stride, rows, size)) ||
                    !aligned(weight, 16) || !aligned(grad_input, 16);

@@ -190,3 +190,19 @@ def test_offsets_of_32_bits_only_where_all_of_them_fit(small_offsets):
                 steps = [1, 1, 1]
                 steps[at] = step
                 assert not small_offsets(rows, *steps) or rows * step < 1 << 31
+
+
+@pytest.mark.parametrize("dtype", [0, 1, 2])
+def test_an_unaligned_workspace_is_refused(dtype):
+    """The kernels write sums of 4 and 8 bytes there."""
+    L = _lib.LIB
+    p, before = ctypes.c_void_p(0x1000), L.optimi_b200_launch_count()
+    for at in (0x1001, 0x1004, 0x1008):
+        rc = L.optimi_b200_rms_norm_backward(p, 64, None, 0, p, 64, p, 2, p, None, 400, 64, dtype, p, p, ctypes.c_void_p(at), 1 << 20, None)
+        assert rc == -3 and b"16-byte aligned" in L.optimi_b200_last_error()
+        if dtype:
+            tokens = 64 * 200  # one tile, cut into slices
+            assert L.optimi_b200_weight_gradient_workspace_bytes(tokens, 64, 64) > 0
+            rc = L.optimi_b200_weight_gradient(p, 64, p, 64, p, 2, None, tokens, 64, 64, dtype, p, ctypes.c_void_p(at), 1 << 30, None)
+            assert rc == -3 and b"16-byte aligned" in L.optimi_b200_last_error()
+    assert L.optimi_b200_launch_count() == before
