@@ -163,8 +163,9 @@ def rms_norm(x: Tensor, weight: Tensor | None = None, residual: Tensor | None = 
     """Root-mean-square norm of ``h = x + residual`` over the last dimension, ``h / sqrt(mean(h**2) + eps) * weight``.
 
     The sum is rounded to `x`'s type before it is normalised, and is returned as the new residual.  `eps` defaults to
-    the type's machine epsilon, as in `torch.nn.RMSNorm`.  Where gradients are wanted the normalised row is kept in 8 bits:
-    the backward pass reads it, and `linear` can share it (`saved`).  `compress=True` keeps it without gradients too.
+    float32's machine epsilon, 2**-23, for all three types, as in `torch.nn.RMSNorm`.  Where gradients are wanted the normalised
+    row is kept in 8 bits: the backward pass reads it, and `linear` can share it (`saved`).  `compress=True` keeps it without
+    gradients too.
     """
     output, new_residual, buffer = _lib.HOST.rms_norm(x, weight, residual, eps, compress)
     if buffer is None:

@@ -236,7 +236,7 @@ std::tuple<Tensor, std::optional<Tensor>, std::optional<Tensor>> rms_norm(const 
     check(name, "residual", residual, &x);
     TORCH_CHECK(residual.sizes() == x.sizes(), name, ": `residual` ", residual.sizes(), " does not match `x` ", x.sizes());
   }
-  const double eps = eps_ ? *eps_ : x.scalar_type() == at::kFloat ? 0x1p-23 : x.scalar_type() == at::kHalf ? 0x1p-10 : 0x1p-7;
+  const double eps = eps_ ? *eps_ : 0x1p-23;  // float32's epsilon for 16-bit types too, as in torch.nn.RMSNorm
   TORCH_CHECK_VALUE(eps >= 0, name, ": eps=", eps, " must not be negative");
   if (at::GradMode::is_enabled() &&
       (x.requires_grad() || (weight.defined() && weight.requires_grad()) || (residual.defined() && residual.requires_grad()))) {

@@ -4,14 +4,13 @@ import ctypes
 
 import pytest
 import torch
+from torch import nn
+
+import test_activations_gpu as common
+from activation_reference import U32, depth, smallest_half_step, unit_roundoff
+from test_activations_gpu import DTYPES, HALF, act, loud, name_of, normal, same_bits
 
 pytestmark = pytest.mark.gpu
-
-
-def act():
-    from optimi_b200 import activations
-
-    return activations
 
 
 def gave_up():
@@ -39,7 +38,7 @@ def test_weight_gradients_one_behind_another():
     assert int(wrong) == 0 and gave_up() == 0
 
 
-@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=name_of)
 def test_exponents_that_are_columns_of_a_table_beyond_32_bits(dtype):
     """Codes close together and exponents 32 KB from row to row: the last rows' lie beyond 2^31 bytes."""
     a = act()
@@ -50,3 +49,40 @@ def test_exponents_that_are_columns_of_a_table_beyond_32_bits(dtype):
     table[:, 5:6] = dense.exponents
     wide = a.CompressedActivation(dense.codes, table[:, 5:6], (rows, cols), dtype)
     assert torch.equal(wide.decompress(), dense.decompress())
+
+
+SCALES = [1e-3, 0.01, 0.02, 1.0, 100.0]  # 0.02: a usual embedding
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=name_of)
+@pytest.mark.parametrize("scale", SCALES)
+def test_norm_with_the_default_epsilon(scale, dtype, monkeypatch):
+    """The formula with 2^-23, forward, kept row and gradients."""
+    monkeypatch.setattr(common, "EPS", 2.0**-23)
+    x, dy = normal((40, 256), dtype, 1, scale), normal((40, 256), dtype, 3, 0.01)
+    w = (1 + 0.1 * normal((256,), torch.float64, 9)).to(dtype)
+    leaves = [t.cuda().requires_grad_() for t in (x, w)]
+    out = act().rms_norm(*leaves)
+    common.check_norm_results(x, w, None, dy, None, (out, *torch.autograd.grad(out.output, leaves, dy.cuda()), None))
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=name_of)
+@pytest.mark.parametrize("scale", SCALES)
+@pytest.mark.parametrize("eps", [None, 1e-6, 1e-2])
+def test_a_prepared_norm_is_the_plain_one(eps, scale, dtype):
+    """Value by value, with gradients and without: both are the formula's, off by the float32 operations before the result and by
+    one rounding to the type here and two at most there (the normalised value, its product with the weight)."""
+    import optimi_b200
+
+    plain = nn.RMSNorm(256, eps=eps)
+    with torch.no_grad():
+        plain.weight.copy_(1 + 0.1 * normal((256,), torch.float64, 9))
+    plain = plain.to(device="cuda", dtype=dtype)
+    x = normal((40, 256), dtype, 1, scale).cuda()
+    want = plain(x).detach().double()
+    prepared = optimi_b200.prepare_for_compressed_activations(plain)
+    bound = want.abs() * (3 * unit_roundoff(dtype) + 2 * (depth(256) / 2 + 6) * U32) * 1.01 + 3 * smallest_half_step(dtype)
+    trained = prepared(x)
+    assert trained.requires_grad and bool(((trained.detach().double() - want).abs() <= bound).all())
+    with torch.no_grad():
+        assert bool(((prepared(x).double() - want).abs() <= bound).all())
