@@ -152,6 +152,11 @@ void refuse_double_backward(const char* name) {
   TORCH_CHECK(!at::GradMode::is_enabled(), name, ": differentiating the backward pass (create_graph=True) is not supported");
 }
 
+void refuse_tangent(const char* name, const char* what, const Tensor& t) {
+  // forward mode needs no input that requires a gradient, so the way past the node would drop the tangent without a word
+  TORCH_CHECK(!t.defined() || !t._fw_grad(0).defined(), name, ": `", what, "` carries a forward-mode tangent; forward-mode differentiation is not supported");
+}
+
 struct Normed {
   Tensor output, sum, buffer;
 };
@@ -238,6 +243,7 @@ std::tuple<Tensor, std::optional<Tensor>, std::optional<Tensor>> rms_norm(const 
   }
   const double eps = eps_ ? *eps_ : 0x1p-23;  // float32's epsilon for 16-bit types too, as in torch.nn.RMSNorm
   TORCH_CHECK_VALUE(eps >= 0, name, ": eps=", eps, " must not be negative");
+  refuse_tangent(name, "x", x), refuse_tangent(name, "weight", weight), refuse_tangent(name, "residual", residual);
   if (at::GradMode::is_enabled() &&
       (x.requires_grad() || (weight.defined() && weight.requires_grad()) || (residual.defined() && residual.requires_grad()))) {
     const variable_list out = RMSNormNode::apply(x, some(weight), some(residual), eps);

@@ -86,3 +86,18 @@ def test_a_prepared_norm_is_the_plain_one(eps, scale, dtype):
     assert trained.requires_grad and bool(((trained.detach().double() - want).abs() <= bound).all())
     with torch.no_grad():
         assert bool(((prepared(x).double() - want).abs() <= bound).all())
+
+
+@pytest.mark.parametrize("carrier", ["x", "weight", "residual"])
+@pytest.mark.parametrize("grads", [True, False])
+def test_forward_mode_tangents_are_refused(carrier, grads):
+    """Not dropped: the result would come without a tangent."""
+    import torch.autograd.forward_ad as fw
+
+    args = dict(x=normal((5, 64), torch.float32, 1).cuda(), weight=torch.ones(64, device="cuda"), residual=normal((5, 64), torch.float32, 2).cuda())
+    want = act().rms_norm(**args)
+    with fw.dual_level(), torch.set_grad_enabled(grads):
+        dual = dict(args, **{carrier: fw.make_dual(args[carrier], torch.ones_like(args[carrier]))})
+        with pytest.raises(RuntimeError, match=f"`{carrier}` carries a forward-mode tangent"):
+            act().rms_norm(**dual)
+        assert same_bits(act().rms_norm(**args).output, want.output)
