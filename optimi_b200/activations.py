@@ -229,7 +229,7 @@ class _CompressedLinear(nn.Linear):
     def forward(self, x: Tensor) -> Tensor:
         casts = torch.is_autocast_enabled("cuda")
         dtype = torch.get_autocast_dtype("cuda") if casts else self.weight.dtype
-        if not (torch.is_grad_enabled() and self.weight.requires_grad and dtype in (torch.bfloat16, torch.float16)):
+        if not (torch.is_grad_enabled() and self.weight.requires_grad and dtype in (torch.bfloat16, torch.float16)) or torch.jit.is_tracing():
             return super().forward(x)
         return linear(x, self.weight, self.bias, saved=_kept(x) if x.dtype == dtype else None)
 
@@ -239,7 +239,7 @@ class _CompressedRMSNorm(nn.RMSNorm):
         w = self.weight
         if not torch.is_grad_enabled() or not (x.requires_grad or (w is not None and w.requires_grad)):
             return super().forward(x)
-        if torch.is_autocast_enabled("cuda") or (w is not None and w.dtype != x.dtype):
+        if torch.is_autocast_enabled("cuda") or torch.jit.is_tracing() or (w is not None and w.dtype != x.dtype):
             return super().forward(x)
         out = rms_norm(x, w, eps=self.eps)
         y = out.output
@@ -252,9 +252,9 @@ def prepare_for_compressed_activations(model: nn.Module) -> nn.Module:
 
     A linear layer that follows such a norm directly shares the norm's 8-bit row; every other one compresses its own
     input.  Layers of other types, subclasses of these two, norms over more than the last dimension, linear layers that
-    compute in float32 and norms under autocast or with a weight of another type stay as they are.  Parameters and
-    `state_dict` do not change, nor do forward results beyond a norm's last bit.  Works with gradient release, gradient
-    accumulation and autocast.
+    compute in float32 and norms under autocast or with a weight of another type stay as they are, and so does every layer
+    under `torch.jit.trace`.  Parameters and `state_dict` do not change, nor do forward results beyond a norm's last bit.  Works
+    with gradient release, gradient accumulation and autocast.
     """
     if hasattr(model, _PREPARED_ATTR):
         raise ValueError("Model is already prepared for compressed activations.")

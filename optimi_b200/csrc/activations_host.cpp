@@ -7,6 +7,7 @@
 #include <ATen/autocast_mode.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 
 #include "../../include/optimi_b200.h"
 
@@ -30,6 +31,11 @@ int dtype_code(at::ScalarType t) {
     case at::kHalf: return OPTIMI_F16;
     default: return -1;
   }
+}
+
+void refuse_tracing(const char* name) {
+  // a trace would record the buffers without the kernel that fills them
+  TORCH_CHECK(!torch::jit::tracer::isTracing(), name, ": the kernels cannot be recorded by torch.jit.trace");
 }
 
 std::string type_name(const Tensor& t) { return "torch." + std::string(c10::getDtypeNames(t.scalar_type()).first); }
@@ -90,6 +96,7 @@ Kept kept_in(const std::vector<Tensor>& tensors, int64_t rows, int64_t cols) {
 }
 
 Tensor compress(const Tensor& x) {
+  refuse_tracing("compress");
   check("compress", "x", x);
   TORCH_CHECK(x.dim() > 0, "compress: `x` must have at least one dimension");
   c10::cuda::CUDAGuard guard(x.device());
@@ -102,6 +109,7 @@ Tensor compress(const Tensor& x) {
 }
 
 Tensor decompress(const std::vector<Tensor>& tensors, const std::vector<int64_t>& shape, at::ScalarType dtype, const std::optional<Tensor>& scale) {
+  refuse_tracing("decompress");
   TORCH_CHECK(tensors[0].is_cuda(), "decompress: `saved` lives on ", tensors[0].device(), "; optimi_b200 takes CUDA tensors only (there is no CPU path)");
   c10::cuda::CUDAGuard guard(tensors[0].device());
   const Tensor out = at::empty(shape, tensors[0].options().dtype(dtype));
@@ -138,6 +146,7 @@ Tensor weight_gradient_of(const Tensor& grad, const std::vector<Tensor>& tensors
 Tensor weight_gradient(const Tensor& grad, const std::vector<Tensor>& tensors, const std::vector<int64_t>& shape, at::ScalarType dtype,
                        const std::optional<Tensor>& scale) {
   const char* name = "weight_gradient";
+  refuse_tracing(name);
   check(name, "grad", grad);
   TORCH_CHECK(grad.scalar_type() != at::kFloat, name, ": `grad` is float32; bfloat16 and float16 are supported");
   TORCH_CHECK(dtype == grad.scalar_type() && tensors[0].device() == grad.device(), name, ": `saved` (torch.", c10::getDtypeNames(dtype).first,
@@ -229,6 +238,7 @@ std::tuple<Tensor, std::optional<Tensor>, std::optional<Tensor>> rms_norm(const 
                                                                           const std::optional<Tensor>& residual_, std::optional<double> eps_,
                                                                           bool keep) {
   const char* name = "rms_norm";
+  refuse_tracing(name);
   const Tensor weight = or_none(weight_), residual = or_none(residual_);
   check(name, "x", x);
   TORCH_CHECK(x.dim() > 0, name, ": `x` must have at least one dimension");
@@ -292,6 +302,7 @@ struct LinearNode : torch::autograd::Function<LinearNode> {
 Tensor linear(const Tensor& x_, const Tensor& weight_, const std::optional<Tensor>& bias_, const std::vector<Tensor>& tensors,
               const std::vector<int64_t>& shape, std::optional<at::ScalarType> dtype, const std::optional<Tensor>& scale) {
   const char* name = "linear";
+  if (at::GradMode::is_enabled()) refuse_tracing(name);
   Tensor x = x_, weight = weight_, bias = or_none(bias_);
   if (at::autocast::is_autocast_enabled(at::kCUDA) && x.is_cuda()) {
     const at::ScalarType to = at::autocast::get_autocast_dtype(at::kCUDA);

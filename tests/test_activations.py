@@ -206,3 +206,29 @@ def test_an_unaligned_workspace_is_refused(dtype):
             rc = L.optimi_b200_weight_gradient(p, 64, p, 64, p, 2, None, tokens, 64, 64, dtype, p, ctypes.c_void_p(at), 1 << 30, None)
             assert rc == -3 and b"16-byte aligned" in L.optimi_b200_last_error()
     assert L.optimi_b200_launch_count() == before
+
+
+@pytest.mark.parametrize("call, modes", [
+    (lambda x: activations.compress(x).codes, (True, False)),
+    (lambda x: activations.decompress(saved_on_cpu()), (True, False)),
+    (lambda x: activations.rms_norm(x).output, (True, False)),
+    (lambda x: activations.linear(x, torch.zeros(8, 40, dtype=torch.bfloat16)), (True,)),  # without gradients it is torch's own
+    (lambda x: activations.weight_gradient(x, saved_on_cpu()), (True, False)),
+], ids=["compress", "decompress", "rms_norm", "linear", "weight_gradient"])  # fmt: skip
+def test_traces_are_refused(call, modes):
+    """A trace would hold the buffers without the kernels that fill them."""
+    for grads in modes:
+        with torch.set_grad_enabled(grads), warnings.catch_warnings():
+            warnings.simplefilter("ignore")
+            with pytest.raises(RuntimeError, match="cannot be recorded by torch.jit.trace"):
+                torch.jit.trace(call, (torch.zeros(4, 40, dtype=torch.bfloat16),), check_trace=False)
+
+
+def test_a_prepared_model_is_traced_as_its_plain_layers():
+    model = nn.Sequential(nn.RMSNorm(40), nn.Linear(40, 8)).bfloat16()
+    x = torch.randn(4, 40).bfloat16()
+    want = model(x)
+    with warnings.catch_warnings():
+        warnings.simplefilter("ignore")
+        traced = torch.jit.trace(optimi_b200.prepare_for_compressed_activations(model), (x,))
+    assert torch.equal(traced(x), want)
