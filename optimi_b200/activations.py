@@ -239,7 +239,7 @@ class _CompressedRMSNorm(nn.RMSNorm):
         w = self.weight
         if not torch.is_grad_enabled() or not (x.requires_grad or (w is not None and w.requires_grad)):
             return super().forward(x)
-        if torch.is_autocast_enabled("cuda") or torch.jit.is_tracing() or (w is not None and w.dtype != x.dtype):
+        if torch.is_autocast_enabled("cuda") or torch.jit.is_tracing() or x.dtype not in _lib.DTYPE_CODE or (w is not None and w.dtype != x.dtype):
             return super().forward(x)
         out = rms_norm(x, w, eps=self.eps)
         y = out.output
@@ -253,7 +253,7 @@ def prepare_for_compressed_activations(model: nn.Module) -> nn.Module:
     A linear layer that follows such a norm directly shares the norm's 8-bit row; every other one compresses its own
     input.  Layers of other types, subclasses of these two, norms over more than the last dimension, linear layers that
     compute in float32 and norms under autocast or with a weight of another type stay as they are, and so does every layer
-    under `torch.jit.trace`.  Parameters and `state_dict` do not change, nor do forward results beyond a norm's last bit.  Works
+    in float64 or under `torch.jit.trace`.  Parameters and `state_dict` do not change, nor do forward results beyond a norm's last bit.  Works
     with gradient release, gradient accumulation and autocast.
     """
     if hasattr(model, _PREPARED_ATTR):

@@ -232,3 +232,13 @@ def test_a_prepared_model_is_traced_as_its_plain_layers():
         warnings.simplefilter("ignore")
         traced = torch.jit.trace(optimi_b200.prepare_for_compressed_activations(model), (x,))
     assert torch.equal(traced(x), want)
+
+
+def test_a_prepared_model_in_float64_stays_as_it_is():
+    for model in (nn.Sequential(nn.RMSNorm(40), nn.Linear(40, 8)), nn.Sequential(nn.RMSNorm(40, elementwise_affine=False), nn.Linear(40, 8))):
+        model.double()
+        x = torch.randn(4, 40, dtype=torch.float64, requires_grad=True)
+        want = torch.autograd.grad(model(x).square().sum(), [x, *model.parameters()])
+        optimi_b200.prepare_for_compressed_activations(model)
+        for got, plain in zip(torch.autograd.grad(model(x).square().sum(), [x, *model.parameters()]), want):
+            assert torch.equal(got, plain)
