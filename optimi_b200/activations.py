@@ -231,6 +231,8 @@ class _CompressedLinear(nn.Linear):
         dtype = torch.get_autocast_dtype("cuda") if casts else self.weight.dtype
         if not (torch.is_grad_enabled() and self.weight.requires_grad and dtype in (torch.bfloat16, torch.float16)) or torch.jit.is_tracing():
             return super().forward(x)
+        if casts and not all(t.is_floating_point() and t.dtype != torch.float64 for t in (x, self.weight)):  # autocast leaves these alone
+            return super().forward(x)
         return linear(x, self.weight, self.bias, saved=_kept(x) if x.dtype == dtype else None)
 
 

@@ -306,8 +306,9 @@ Tensor linear(const Tensor& x_, const Tensor& weight_, const std::optional<Tenso
   Tensor x = x_, weight = weight_, bias = or_none(bias_);
   if (at::autocast::is_autocast_enabled(at::kCUDA) && x.is_cuda()) {
     const at::ScalarType to = at::autocast::get_autocast_dtype(at::kCUDA);
-    x = x.to(to), weight = weight.to(to);
-    if (bias.defined()) bias = bias.to(to);
+    const auto cast = [&](const Tensor& t) { return t.is_cuda() && t.is_floating_point() && t.scalar_type() != at::kDouble ? t.to(to) : t; };
+    x = cast(x), weight = cast(weight);
+    if (bias.defined()) bias = cast(bias);
   }
   check(name, "x", x);
   check(name, "weight", weight, &x);

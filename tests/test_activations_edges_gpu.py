@@ -101,3 +101,27 @@ def test_forward_mode_tangents_are_refused(carrier, grads):
         with pytest.raises(RuntimeError, match=f"`{carrier}` carries a forward-mode tangent"):
             act().rms_norm(**dual)
         assert same_bits(act().rms_norm(**args).output, want.output)
+
+
+def test_autocast_leaves_float64_alone():
+    """As it does with the plain layer."""
+    import optimi_b200
+
+    model, x = nn.Linear(64, 32).cuda().double(), normal((5, 64), torch.float64, 1).cuda().requires_grad_()
+    leaves = [x, *model.parameters()]
+    with torch.autocast("cuda", dtype=torch.bfloat16):
+        want = model(x)
+        grads = torch.autograd.grad(want.square().sum(), leaves)
+        got = optimi_b200.prepare_for_compressed_activations(model)(x)
+        assert got.dtype == torch.float64 and torch.equal(got, want)
+        for a, b in zip(torch.autograd.grad(got.square().sum(), leaves), grads):
+            assert torch.equal(a, b)
+        with pytest.raises(RuntimeError, match="unsupported dtype torch.float64"):
+            act().linear(x, model.weight)
+        with pytest.raises(RuntimeError, match="does not match"):
+            act().linear(x.bfloat16(), model.weight)
+        with pytest.raises(RuntimeError, match="unsupported dtype"):
+            act().linear(torch.zeros(5, 64, dtype=torch.int32, device="cuda"), model.weight.float())
+        # float32 and the other 16-bit type are cast, the layer's as the operator's
+        y = act().linear(x.float(), model.weight.half(), model.bias.float())
+        assert same_bits(y.detach(), nn.functional.linear(x.bfloat16(), model.weight.half().bfloat16(), model.bias.bfloat16()).detach())
