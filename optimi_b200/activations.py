@@ -67,7 +67,7 @@ class CompressedActivation:
         if codes.device != exponents.device:
             raise ValueError(f"codes are on {codes.device} and exponents on {exponents.device}")
         if rows and cols:
-            if codes.stride(1) != 1 or exponents.stride(1) != 1 or (rows > 1 and codes.stride(0) % GROUP) or codes.data_ptr() % 16:
+            if codes.stride(1) != 1 or (exponents.shape[1] > 1 and exponents.stride(1) != 1) or (rows > 1 and codes.stride(0) % GROUP) or codes.data_ptr() % 16:
                 raise ValueError("rows of codes and exponents must be contiguous, codes 16-byte aligned with a pitch that is a multiple of 32")
             if rows > 1 and (codes.stride(0) < padded or exponents.stride(0) < padded // GROUP):
                 raise ValueError("rows of codes and exponents must not overlap")

@@ -92,6 +92,7 @@ Kept kept_in(const Tensor& buffer, int64_t rows, int64_t cols) {
 
 Kept kept_in(const std::vector<Tensor>& tensors, int64_t rows, int64_t cols) {
   if (tensors.size() == 1) return kept_in(tensors[0], rows, cols);
+  if (rows <= 1) return {tensors[0].data_ptr(), groups_of(cols) * kGroup, tensors[1].data_ptr(), groups_of(cols)};  // strides of one row mean nothing
   return {tensors[0].data_ptr(), tensors[0].stride(0), tensors[1].data_ptr(), tensors[1].stride(0)};
 }
 

@@ -125,3 +125,30 @@ def test_autocast_leaves_float64_alone():
         # float32 and the other 16-bit type are cast, the layer's as the operator's
         y = act().linear(x.float(), model.weight.half(), model.bias.float())
         assert same_bits(y.detach(), nn.functional.linear(x.bfloat16(), model.weight.half().bfloat16(), model.bias.bfloat16()).detach())
+
+
+@pytest.mark.parametrize("dtype", HALF, ids=name_of)
+@pytest.mark.parametrize("cols", [32, 20, 45, 64])
+def test_strides_without_meaning(cols, dtype):
+    """Those of one row, and that of one group: any number may stand there."""
+    a = act()
+    x, grad = normal((1, cols), dtype, 1).cuda(), normal((1, 24), dtype, 2).cuda()
+    dense = a.compress(x)
+    padded, groups = dense.codes.shape[1], dense.exponents.shape[1]
+    wider = torch.zeros((1, padded + 16), dtype=torch.int8, device="cuda")
+    wider[:, :padded] = dense.codes
+    upright = torch.empty_like(dense.codes[0]).copy_(dense.codes[0]).view(-1, 1).t(), dense.exponents[0].clone().view(-1, 1).t()
+    assert upright[0].stride() == (1, 1)
+    odd = dense.codes.as_strided((1, padded), (7, 1)), dense.exponents.as_strided((1, groups), (0, 1))
+    for codes, exponents in [(wider, dense.exponents), upright, odd]:
+        saved = a.CompressedActivation(codes, exponents, (cols,), dtype)
+        assert same_bits(saved.decompress(), dense.decompress()[0])
+        assert same_bits(a.weight_gradient(grad, saved), a.weight_gradient(grad, dense))
+        w = normal((24, cols), dtype, 3).cuda().requires_grad_()
+        assert same_bits(torch.autograd.grad(a.linear(x, w, saved=saved), w, grad)[0], a.weight_gradient(grad, dense))
+    if groups == 1:
+        many = a.compress(normal((9, cols), dtype, 4).cuda())
+        lying = torch.zeros((1, 9), dtype=torch.uint8, device="cuda")
+        lying[0] = many.exponents[:, 0]
+        assert lying.t().stride() == (1, 9)
+        assert same_bits(a.CompressedActivation(many.codes, lying.t(), (9, cols), dtype).decompress(), many.decompress())
