@@ -294,7 +294,7 @@ struct LinearNode : torch::autograd::Function<LinearNode> {
     if (grad.defined()) {
       if (ctx->needs_input_grad(0)) dx = at::matmul(grad, kept[0]);
       if (ctx->needs_input_grad(1)) dw = weight_gradient_of(grad, {kept.begin() + 2, kept.end()}, ctx->saved_data["channels"].toInt(), kept[1]);
-      if (ctx->saved_data["bias"].toBool() && ctx->needs_input_grad(2)) db = grad.reshape({-1, grad.size(-1)}).sum(0);
+      if (ctx->saved_data["bias"].toBool() && ctx->needs_input_grad(2)) db = grad.reshape({rows_of(grad.sizes()), grad.size(-1)}).sum(0);
     }
     return {dx, dw, db, Tensor()};
   }

@@ -152,3 +152,12 @@ def test_strides_without_meaning(cols, dtype):
         lying[0] = many.exponents[:, 0]
         assert lying.t().stride() == (1, 9)
         assert same_bits(a.CompressedActivation(many.codes, lying.t(), (9, cols), dtype).decompress(), many.decompress())
+
+
+@pytest.mark.parametrize("shape", [(5, 40, 0), (5, 0, 7), (0, 40, 7), (0, 0, 0)], ids=str)
+def test_a_linear_layer_without_tokens_channels_or_outputs(shape):
+    tokens, channels, outputs = shape
+    x, w, b = (torch.ones(s, dtype=torch.bfloat16, device="cuda", requires_grad=True) for s in ((tokens, channels), (outputs, channels), (outputs,)))
+    y = act().linear(x, w, b)
+    for got, want in zip(torch.autograd.grad(y, (x, w, b), torch.ones_like(y)), torch.autograd.grad(nn.functional.linear(x, w, b), (x, w, b), torch.ones_like(y))):
+        assert got.shape == want.shape and got.dtype == want.dtype and torch.equal(got, want)
