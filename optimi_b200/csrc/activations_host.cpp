@@ -67,6 +67,9 @@ Tensor as_rows(const Tensor& given) {
   return t;
 }
 
+// A norm's weight or the scale of the channels: its values one after another in memory (not those of a lazily negated view).
+Tensor as_channels(const Tensor& t) { return t.defined() ? t.detach().resolve_neg().contiguous() : Tensor(); }
+
 Tensor dense_like(const Tensor& t) { return at::empty(t.sizes(), t.options().memory_format(at::MemoryFormat::Contiguous)); }
 Tensor bytes(int64_t n, const Tensor& like) { return at::empty({n}, like.options().dtype(at::kByte)); }
 void* stream_of(const Tensor& t) { return c10::cuda::getCurrentCUDAStream(t.device().index()).stream(); }
@@ -114,7 +117,7 @@ Tensor decompress(const std::vector<Tensor>& tensors, const std::vector<int64_t>
   TORCH_CHECK(tensors[0].is_cuda(), "decompress: `saved` lives on ", tensors[0].device(), "; optimi_b200 takes CUDA tensors only (there is no CPU path)");
   c10::cuda::CUDAGuard guard(tensors[0].device());
   const Tensor out = at::empty(shape, tensors[0].options().dtype(dtype));
-  const Tensor s = scale ? scale->detach().contiguous() : Tensor();
+  const Tensor s = as_channels(or_none(scale));
   const int64_t rows = rows_of(shape), cols = shape.back();
   const Kept k = kept_in(tensors, rows, cols);
   check_rc(optimi_b200_decompress(k.codes, k.pitch, k.exponents, k.epitch, ptr(s), rows, cols, dtype_code(dtype), out.data_ptr(), stream_of(out)));
@@ -137,7 +140,7 @@ Tensor weight_gradient_of(const Tensor& grad, const std::vector<Tensor>& tensors
   const Tensor dw = at::empty({outputs, channels}, m.options());
   const size_t need = optimi_b200_weight_gradient_workspace_bytes(rows, outputs, channels);
   const Tensor workspace = need ? bytes((int64_t)need, m) : Tensor();
-  const Tensor s = scale.defined() ? scale.detach().contiguous() : Tensor();
+  const Tensor s = as_channels(scale);
   const Kept k = kept_in(tensors, rows, channels);
   check_rc(optimi_b200_weight_gradient(m.data_ptr(), stride, k.codes, k.pitch, k.exponents, k.epitch, ptr(s), rows, outputs, channels, code,
                                        dw.data_ptr(), ptr(workspace), need, stream));
@@ -174,7 +177,7 @@ struct Normed {
 Normed norm_forward(const Tensor& x, const Tensor& weight, const Tensor& residual, double eps, bool keep) {
   c10::cuda::CUDAGuard guard(x.device());
   const Tensor m = as_rows(x), r = residual.defined() ? as_rows(residual) : Tensor();
-  const Tensor w = weight.defined() ? weight.detach().contiguous() : Tensor();
+  const Tensor w = as_channels(weight);
   const int64_t rows = m.size(0), cols = m.size(1);
   Normed out;
   out.output = dense_like(x);
@@ -220,7 +223,7 @@ struct RMSNormNode : torch::autograd::Function<RMSNormNode> {
     }
     c10::cuda::CUDAGuard guard(grad.device());
     const Tensor g = as_rows(grad), s = grad_sum.defined() ? as_rows(grad_sum) : Tensor();
-    const Tensor w = weight.defined() ? weight.detach().contiguous() : Tensor();
+    const Tensor w = as_channels(weight);
     const int64_t rows = g.size(0), cols = g.size(1);
     const int code = dtype_code(grad.scalar_type());
     const Tensor dx = need_x || need_r ? dense_like(grad) : Tensor(), dw = need_w ? at::empty({cols}, g.options()) : Tensor();

@@ -161,3 +161,25 @@ def test_a_linear_layer_without_tokens_channels_or_outputs(shape):
     y = act().linear(x, w, b)
     for got, want in zip(torch.autograd.grad(y, (x, w, b), torch.ones_like(y)), torch.autograd.grad(nn.functional.linear(x, w, b), (x, w, b), torch.ones_like(y))):
         assert got.shape == want.shape and got.dtype == want.dtype and torch.equal(got, want)
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=name_of)
+def test_lazily_negated_weights_and_scales(dtype):
+    """Views whose memory holds the opposite, as the imaginary part of a conjugate is."""
+    a = act()
+    x, r, dy, w = (normal(s, dtype, i).cuda() for i, s in enumerate([(6, 40), (6, 40), (6, 40), (40,)]))
+    negated = torch._neg_view(-w)
+    assert negated.is_neg() and negated.is_contiguous() and same_bits(negated.clone(), w)
+    saved = a.compress(x)
+    assert same_bits(a.CompressedActivation(saved.codes, saved.exponents, (6, 40), dtype, negated).decompress(),
+                     a.CompressedActivation(saved.codes, saved.exponents, (6, 40), dtype, w).decompress())  # fmt: skip
+    results = []
+    for weight in (negated, w):
+        leaves = [t.detach().requires_grad_() for t in (x, weight, r)]
+        out = a.rms_norm(*leaves)
+        results.append([out.output.detach(), out.saved.decompress(), *torch.autograd.grad(out.output, leaves, dy)])
+        results[-1].append(a.rms_norm(torch._neg_view(-x), weight, torch._neg_view(-r)).output)
+        if dtype != torch.float32:
+            results[-1].append(a.weight_gradient(torch._neg_view(-dy), out.saved))
+    for got, want in zip(*results):
+        assert same_bits(got, want)
