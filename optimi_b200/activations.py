@@ -20,6 +20,7 @@ activation in place of the original.  CUDA tensors only, like the optimizers.
 
 from __future__ import annotations
 
+from collections import OrderedDict
 from collections.abc import Callable, Sequence
 from typing import Any, NamedTuple
 from warnings import warn
@@ -219,10 +220,25 @@ def checkpoint(function: Callable, *args: Any, **kwargs: Any):
 # ---------------------------------------------------------------------------------------------
 
 
+class _Kept:
+    """A norm's 8-bit row, on the norm's output, and what tells whether that is still the tensor it was."""
+
+    __slots__ = ("saved", "version", "address", "shape")
+
+    def __init__(self, saved: CompressedActivation, y: Tensor):
+        self.saved, self.version, self.address, self.shape = saved, y._version, y.data_ptr(), y.shape
+
+    def __reduce__(self):
+        # a copy or a file of the output has no part in it (and loads with weights_only)
+        return OrderedDict, ()
+
+
 def _kept(x: Tensor) -> CompressedActivation | None:
     """The 8-bit form a norm attached to this very tensor, unless the tensor was written to or given other memory since."""
     kept = getattr(x, _KEPT_ATTR, None)
-    return kept[0] if kept is not None and kept[1:] == (x._version, x.data_ptr(), x.shape) else None
+    if type(kept) is not _Kept or (kept.version, kept.address, kept.shape) != (x._version, x.data_ptr(), x.shape):
+        return None
+    return kept.saved
 
 
 class _CompressedLinear(nn.Linear):
@@ -245,7 +261,7 @@ class _CompressedRMSNorm(nn.RMSNorm):
             return super().forward(x)
         out = rms_norm(x, w, eps=self.eps)
         y = out.output
-        setattr(y, _KEPT_ATTR, (out.saved, y._version, y.data_ptr(), y.shape))
+        setattr(y, _KEPT_ATTR, _Kept(out.saved, y))
         return y
 
 

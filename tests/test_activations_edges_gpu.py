@@ -1,6 +1,8 @@
 """Activation operators at the edges of what they accept, against their definitions in 64 bits (activation_reference.py)."""
 
+import copy
 import ctypes
+import io
 
 import pytest
 import torch
@@ -183,3 +185,22 @@ def test_lazily_negated_weights_and_scales(dtype):
             results[-1].append(a.weight_gradient(torch._neg_view(-dy), out.saved))
     for got, want in zip(*results):
         assert same_bits(got, want)
+
+
+def test_a_norms_output_is_saved_and_copied_without_its_row():
+    import optimi_b200
+
+    model = nn.Sequential(nn.RMSNorm(64), nn.Linear(64, 32, bias=False)).to(device="cuda", dtype=torch.bfloat16)
+    optimi_b200.prepare_for_compressed_activations(model)
+    y = model[0](normal((40, 64), torch.bfloat16, 1).cuda())
+    files = [io.BytesIO(), io.BytesIO()]
+    torch.save(y, files[0])
+    torch.save(y.detach().clone(), files[1])
+    assert abs(files[0].tell() - files[1].tell()) < 1000  # the row is 40 * 66 bytes
+    files[0].seek(0)
+    loaded = torch.load(files[0], weights_only=True)
+    assert same_bits(loaded.detach(), y.detach())
+    dy = normal((40, 32), torch.bfloat16, 2).cuda()
+    for other in (loaded, copy.copy(y)):
+        (dw,) = torch.autograd.grad(model[1](other), model[1].weight, dy)
+        assert same_bits(dw, act().weight_gradient(dy, act().compress(other.detach())))
