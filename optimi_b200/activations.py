@@ -221,12 +221,17 @@ def checkpoint(function: Callable, *args: Any, **kwargs: Any):
 
 
 class _Kept:
-    """A norm's 8-bit row, on the norm's output, and what tells whether that is still the tensor it was."""
+    """A norm's 8-bit row, on the norm's output, and what tells whether that is still the tensor it was.
 
-    __slots__ = ("saved", "version", "address", "shape")
+    The row is shared only where saved tensors take the way they took in the norm: a block that is run again in the backward
+    pass gets the output of a norm outside as a tensor of its own, without the row, and has to save the same both times.
+    """
+
+    __slots__ = ("saved", "version", "address", "shape", "hook")
 
     def __init__(self, saved: CompressedActivation, y: Tensor):
         self.saved, self.version, self.address, self.shape = saved, y._version, y.data_ptr(), y.shape
+        self.hook = _lib.HOST.saving_hook()
 
     def __reduce__(self):
         # a copy or a file of the output has no part in it (and loads with weights_only)
@@ -238,7 +243,7 @@ def _kept(x: Tensor) -> CompressedActivation | None:
     kept = getattr(x, _KEPT_ATTR, None)
     if type(kept) is not _Kept or (kept.version, kept.address, kept.shape) != (x._version, x.data_ptr(), x.shape):
         return None
-    return kept.saved
+    return kept.saved if kept.hook is _lib.HOST.saving_hook() else None
 
 
 class _CompressedLinear(nn.Linear):

@@ -4,9 +4,11 @@
 // kernels of a small layer take.
 #include <torch/extension.h>
 
+#include <ATen/SavedTensorHooks.h>
 #include <ATen/autocast_mode.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
+#include <torch/csrc/PyInterpreter.h>
 #include <torch/csrc/jit/frontend/tracer.h>
 
 #include "../../include/optimi_b200.h"
@@ -331,6 +333,12 @@ Tensor linear(const Tensor& x_, const Tensor& weight_, const std::optional<Tenso
   return LinearNode::apply(x, weight, some(bias), Saved{tensors, or_none(scale)});
 }
 
+// The function that tensors saved for a backward pass go through now (None: they are kept as they are).
+py::object saving_hook() {
+  const auto hooks = at::SavedTensorDefaultHooks::get_hooks();
+  return hooks ? py::reinterpret_borrow<py::object>(hooks->first.ptr(getPyInterpreter())) : py::none();
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -339,4 +347,5 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("weight_gradient", torch::wrap_pybind_function_no_gil(weight_gradient));
   m.def("rms_norm", torch::wrap_pybind_function_no_gil(rms_norm));
   m.def("linear", torch::wrap_pybind_function_no_gil(linear));
+  m.def("saving_hook", saving_hook);
 }

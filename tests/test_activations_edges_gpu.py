@@ -204,3 +204,72 @@ def test_a_norms_output_is_saved_and_copied_without_its_row():
     for other in (loaded, copy.copy(y)):
         (dw,) = torch.autograd.grad(model[1](other), model[1].weight, dy)
         assert same_bits(dw, act().weight_gradient(dy, act().compress(other.detach())))
+
+
+def through_torch(function, x):
+    return torch.utils.checkpoint.checkpoint(function, x, use_reentrant=False)
+
+
+def through_torch_on_cpu(function, x):
+    with torch.autograd.graph.save_on_cpu():
+        return through_torch(function, x)
+
+
+def through_eight_bits(function, x):
+    return act().checkpoint(function, x)
+
+
+def through_both(function, x):
+    return through_eight_bits(lambda t: through_torch(function, t), x)
+
+
+@pytest.mark.parametrize("through", [through_torch, through_torch_on_cpu, through_eight_bits, through_both])
+def test_recomputed_layers_behind_a_norm(through):
+    """The norm within the block that is run again: its row is shared, as without recomputation.  The norm before it: the layer keeps
+    its input itself, in both runs."""
+    import optimi_b200
+
+    torch.manual_seed(0)
+    norm, layers = nn.RMSNorm(64), nn.ModuleList([nn.Linear(64, 32), nn.Linear(64, 32)])
+    model = nn.ModuleList([norm, layers]).to(device="cuda", dtype=torch.bfloat16)
+    optimi_b200.prepare_for_compressed_activations(model)
+    a = act()
+    x = a.decompress(a.compress(normal((40, 64), torch.bfloat16, 1).cuda()))  # 8 bits hold it exactly
+    x.requires_grad_()
+    leaves, dy = [x, *model.parameters()], normal((40, 32), torch.bfloat16, 2).cuda()
+
+    def both(t):
+        y = norm(t)
+        return layers[0](y) + layers[1](y)
+
+    plain = both(x * 1.0)
+    want = torch.autograd.grad(plain, leaves, dy)
+    again = through(both, x * 1.0)
+    assert same_bits(again.detach(), plain.detach())
+    for got, expected in zip(torch.autograd.grad(again, leaves, dy), want):
+        assert same_bits(got, expected)
+
+    y = norm(x * 1.0)
+    outside = through(lambda t: layers[0](t) + layers[1](t), y)
+    assert same_bits(outside.detach(), plain.detach())
+    got = torch.autograd.grad(outside, leaves, dy)
+    for i, layer in enumerate(layers):
+        assert same_bits(got[2 + 2 * i], a.weight_gradient(dy, a.compress(y.detach())))
+        assert same_bits(got[3 + 2 * i], want[3 + 2 * i])
+    assert same_bits(got[0], want[0]) and same_bits(got[1], want[1])
+
+
+def test_a_norm_and_a_layer_under_the_same_hooks_share_the_row():
+    import optimi_b200
+
+    model = nn.Sequential(nn.RMSNorm(64), nn.Linear(64, 32, bias=False)).to(device="cuda", dtype=torch.bfloat16)
+    optimi_b200.prepare_for_compressed_activations(model)
+    x, dy = normal((40, 64), torch.bfloat16, 1).cuda(), normal((40, 32), torch.bfloat16, 2).cuda()
+    row = act().rms_norm(x, model[0].weight, compress=True).saved
+    with torch.autograd.graph.save_on_cpu():
+        out = model(x)
+    assert same_bits(torch.autograd.grad(out, model[1].weight, dy)[0], act().weight_gradient(dy, row))
+    y = model[0](x)
+    with torch.autograd.graph.save_on_cpu():
+        out = model[1](y)
+    assert same_bits(torch.autograd.grad(out, model[1].weight, dy)[0], act().weight_gradient(dy, act().compress(y.detach())))
