@@ -9,6 +9,7 @@ from __future__ import annotations
 
 import ctypes
 import importlib.util
+import threading
 
 import torch
 
@@ -56,7 +57,7 @@ def _load() -> ctypes.CDLL:
     path = _build.LIB
     if not _build.up_to_date():
         # not built yet, or built from other sources: build now (needs nvcc), else fail loudly
-        path = _build.build(force=True)
+        path = _build.build(host=False)
     lib = ctypes.CDLL(path)
     for name, argtypes in SIGNATURES.items():
         fn = getattr(lib, name)
@@ -111,7 +112,9 @@ def _load() -> ctypes.CDLL:
 
 
 def _load_host():
-    """The C++ module beside the library (optimi_b200/csrc/activations_host.cpp); it links against the library loaded above."""
+    """The C++ module beside the library (optimi_b200/csrc/activations_host.cpp); it links against the library loaded below."""
+    if not _build.host_up_to_date():
+        _build.build(library=False)
     spec = importlib.util.spec_from_file_location("_host", _build.HOST_LIB)
     module = importlib.util.module_from_spec(spec)
     spec.loader.exec_module(module)
@@ -120,7 +123,17 @@ def _load_host():
 
 LIB = _load()
 LIB_PATH = _build.LIB
-HOST = _load_host()
+_host_lock = threading.Lock()
+
+
+def __getattr__(name: str):
+    # HOST, on its first use: it is built for the installed torch, which the optimizers do not need
+    if name != "HOST":
+        raise AttributeError(f"module {__name__!r} has no attribute {name!r}")
+    with _host_lock:
+        if "HOST" not in globals():
+            globals()["HOST"] = _load_host()
+    return globals()["HOST"]
 
 
 class peer_push:
