@@ -6,6 +6,7 @@
 
 #include <ATen/SavedTensorHooks.h>
 #include <ATen/autocast_mode.h>
+#include <c10/cuda/CUDACachingAllocator.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/PyInterpreter.h>
@@ -330,6 +331,9 @@ Tensor linear(const Tensor& x_, const Tensor& weight_, const std::optional<Tenso
                 ") does not stand for `x` (", x.sizes(), ", ", type_name(x), ", ", x.device(), ")");
   if (!at::GradMode::is_enabled()) return at::linear(x, weight, some(bias));
   c10::cuda::CUDAGuard guard(x.device());
+  // The backward pass reads the row on this stream, and whoever made it on another one does not know of that: a prepared norm's
+  // row is not even seen by the caller.
+  for (const Tensor& t : tensors) c10::cuda::CUDACachingAllocator::recordStream(t.storage().data_ptr(), c10::cuda::getCurrentCUDAStream(x.device().index()));
   return LinearNode::apply(x, weight, some(bias), Saved{tensors, or_none(scale)});
 }
 

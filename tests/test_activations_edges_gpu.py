@@ -273,3 +273,37 @@ def test_a_norm_and_a_layer_under_the_same_hooks_share_the_row():
     with torch.autograd.graph.save_on_cpu():
         out = model[1](y)
     assert same_bits(torch.autograd.grad(out, model[1].weight, dy)[0], act().weight_gradient(dy, act().compress(y.detach())))
+
+
+@pytest.mark.parametrize("prepared", [True, False], ids=["prepared layers", "operators"])
+def test_a_row_made_on_one_stream_and_read_on_another(prepared):
+    """The weight gradient alone is asked for, late on the layer's stream; the graph and the row are dropped at once, and the norm's
+    stream takes memory of the row's size and writes to it."""
+    import optimi_b200
+
+    a = act()
+    norm, layer = nn.RMSNorm(512), nn.Linear(512, 256, bias=False)
+    model = nn.Sequential(norm, layer).to(device="cuda", dtype=torch.bfloat16)
+    if prepared:
+        optimi_b200.prepare_for_compressed_activations(model)
+    x, dy = normal((3000, 512), torch.bfloat16, 1).cuda().requires_grad_(), normal((3000, 256), torch.bfloat16, 2).cuda()
+    row = a.rms_norm(x.detach(), norm.weight.detach(), eps=2.0**-23, compress=True).saved
+    want, size = a.weight_gradient(dy, row), row._tensors()[0].numel()
+    del row
+    side = torch.cuda.Stream()
+    for _ in range(3):
+        if prepared:
+            y, saved = norm(x), None
+        else:
+            y, _, saved = a.rms_norm(x, norm.weight)
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            y.record_stream(side), dy.record_stream(side)
+            out = layer(y) if prepared else a.linear(y, layer.weight, saved=saved)
+            torch.cuda._sleep(20_000_000)  # about ten milliseconds
+            (dw,) = torch.autograd.grad(out, layer.weight, dy)
+        del y, saved, out
+        taken = [torch.full((size,), 0x55, dtype=torch.uint8, device="cuda") for _ in range(8)]
+        torch.cuda.synchronize()
+        assert same_bits(dw, want)
+        del taken
