@@ -3,6 +3,7 @@
 import copy
 import ctypes
 import io
+import threading
 
 import pytest
 import torch
@@ -307,3 +308,34 @@ def test_a_row_made_on_one_stream_and_read_on_another(prepared):
         torch.cuda.synchronize()
         assert same_bits(dw, want)
         del taken
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=name_of)
+def test_norms_from_two_threads(dtype):
+    """Forward, kept row and gradients on two streams at once: the bits of the calls alone."""
+    a = act()
+    leaves = [t.cuda().requires_grad_() for t in (loud((700, 512), dtype, 1), (1 + 0.1 * normal((512,), torch.float64, 9)).to(dtype), normal((700, 512), dtype, 2))]
+    grads = normal((700, 512), dtype, 3).cuda(), normal((700, 512), dtype, 4).cuda()
+
+    def call():
+        out = a.rms_norm(*leaves)
+        return [out.output.detach(), out.residual.detach(), out.saved.codes, out.saved.exponents, *torch.autograd.grad(out[:2], leaves, grads)]
+
+    want = [t.clone() for t in call()]
+    torch.cuda.synchronize()
+    failures = []
+
+    def work():
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(30):
+                    failures.extend(i for i, (got, expected) in enumerate(zip(call(), want)) if not torch.equal(got, expected))
+        except RuntimeError as e:
+            failures.append(e)
+
+    threads = [threading.Thread(target=work) for _ in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failures
