@@ -273,8 +273,10 @@ class _CompressedRMSNorm(nn.RMSNorm):
 def prepare_for_compressed_activations(model: nn.Module) -> nn.Module:
     """Makes the `nn.Linear` and `nn.RMSNorm` layers of `model` keep their activations in 8 bits while gradients are recorded.
 
-    A linear layer that follows such a norm directly shares the norm's 8-bit row; every other one compresses its own
-    input.  Layers of other types, subclasses of these two, norms over more than the last dimension, linear layers that
+    A linear layer that follows such a norm directly shares the norm's 8-bit row, unless only one of the two is in a block that is
+    recomputed; every other one compresses its own input, so that layers which share an input that no such norm made keep it
+    once each (`linear` with one `compress(x)` for all of them does not).  What is written to a norm's output past autograd
+    (`.data`, raw pointers) is not seen by the row.  Layers of other types, subclasses of these two, norms over more than the last dimension, linear layers that
     compute in float32 and norms under autocast or with a weight of another type stay as they are, and so does every layer
     in float64 or under `torch.jit.trace`.  Parameters and `state_dict` do not change, nor do forward results beyond a norm's last bit.  Works
     with gradient release, gradient accumulation and autocast.

@@ -8,9 +8,9 @@
 // bytes (one read of 8 bits a value) where a 16-bit copy beside dY would be written and then read again.
 // code * 2^k has 7 bits and fits bf16 and fp16 exactly, so the products are those of the restored activation.
 //
-// What bounds it: the tensor cores and the card's power.  8192 tokens, 14336 outputs x 4096 channels, bf16: 615 us alone
-// (1564 TFLOP/s, 0.94 of the measured product rate) and 735 to 755 us in a long run, where the clock falls to 1.3 GHz (a 16-bit
-// product of the same sizes by the vendor's library: 618 and 716 us there).  4096 x 1024: 58 us, 64 tiles on 74 pairs, the
+// What bounds it: the tensor cores and the card's power.  8192 tokens, 14336 outputs x 4096 channels, bf16: 615 to 625 us alone
+// (1540 to 1564 TFLOP/s, 0.93 to 0.94 of the measured product rate) and 735 to 755 us in a long run, where the clock falls to 1.3 GHz
+// (a 16-bit product of the same sizes by the vendor's library: 612 to 618 and 716 to 723 us there).  4096 x 1024: 58 to 60 us, 64 tiles on 74 pairs, the
 // tensor cores of those 94 % busy.  With few tokens it is the results' way to memory (64 tokens, 4096 x 4096: 23 us).
 #include "activation_common.cuh"
 
